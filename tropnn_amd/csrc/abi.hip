@@ -16,6 +16,7 @@
 #include <string>
 
 #include "launch.hpp"
+#include "logits.hpp"
 
 namespace {
 
@@ -158,6 +159,21 @@ void arm_events(int kernel, hipEvent_t start, hipEvent_t stop) {
     g_armed[kernel].start = start;
     g_armed[kernel].stop = stop;
 }
+
+}  // namespace tropnn
+
+namespace tropnn {
+
+int abi_fail(int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+int abi_ok() { return ok(); }
+int abi_hip_fail(const char *where, hipError_t e) { return hip_fail(where, e); }
 
 }  // namespace tropnn
 
