@@ -6,14 +6,15 @@
 // complement of its index: all of a row's are different, and "the first k",
 // "the shortest prefix of that mass" are the logits at or above one of them.
 //
-// Most of a row is far from any cut, so it is read once, as a stream, against
-// a bound: the k-th largest of the maxima of the first slab's pieces (16
-// bytes each) cannot be above the k-th largest logit. What is below the bound
-// costs one comparison a piece; the few logits at or above it are collected
-// in LDS (collect), where the bound is raised when they become many, and
-// sorted there. Rows whose logits defeat that (thousands of equal ones at the
-// bound, rising rows) take the exact search instead: a cut is found digit by
-// digit, from the mass (a count, or the sampling weights as integers) of every
+// Most of a row is far from its k-th logit, so it is read once, as a stream,
+// against a bound: the k-th largest of the maxima of the first slab's pieces
+// (16 bytes each) cannot be above the k-th largest logit. A piece below the
+// bound costs one comparison; the few others are put aside in LDS (collect)
+// and end as a short list that is sorted there. A share of the mass needs the
+// whole row's: the weights are summed by exponent in LDS, which gives the mass
+// and the narrow range of logits in which the prefix ends. Rows that defeat
+// these (thousands of equal logits at the bound, rising rows) take the exact
+// search instead: a cut is found digit by digit, from the mass (a count, or the sampling weights as integers) of every
 // value of the key's next eight bits among the logits that share the digits
 // before (find_cut). Integer sums do not depend on their order, so neither
 // does a cut or a drawn token.
@@ -26,7 +27,6 @@ constexpr int kBins = 256;
 constexpr int kSlab = 8;        // pieces of a thread that are in flight together
 constexpr int kMassBins = 2048; // of a row's weights, by exponent
 constexpr int kMaxSlabs = 64;
-constexpr int kGuess = 128;     // logits to collect where no top_k says how many
 constexpr float kFixed = 1099511627776.f;  // 2^40: sampling weights are multiples of 2^-40
 
 using u64 = unsigned long long;
@@ -46,6 +46,15 @@ __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_el
 // Logits that a workgroup can collect: eight a thread.
 template <int THREADS>
 constexpr int kList = THREADS < 512 ? 8 * THREADS : 4096;
+
+// The largest logit of a piece, NaN if one is.
+template <typename T>
+__device__ __forceinline__ float piece_most(const words4 &w) {
+    float most = piece_value<T>(w, 0);
+#pragma unroll
+    for (int i = 1; i < kPerLoad<T>; ++i) most = nan_max(most, piece_value<T>(w, i));
+    return most;
+}
 
 template <int THREADS>
 struct Shared {
@@ -310,121 +319,149 @@ __device__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
     return bound;
 }
 
-// Drops collected logits that cannot be among the first k (n > k of them),
-// after dropped(value); returns how many are left.
-template <int THREADS, typename D>
-__device__ int shrink_list(int n, int k, float &bound, D &&dropped, Shared<THREADS> &sh) {
-    constexpr int kOwn = kList<THREADS> / THREADS;
-    u64 own[kOwn];
+// The sum of all threads' parts (not negative), the same bits however they are
+// dealt to the threads: as integers in units of 2^-40 of the largest. NaN where
+// one is NaN or infinite.
+template <int COUNT, int THREADS>
+__device__ float sum_in_any_order(const float (&parts)[COUNT], Shared<THREADS> &sh) {
+    uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        const int i = j * THREADS + static_cast<int>(threadIdx.x);
-        own[j] = i < n ? sh.list[i] : 0;
-    }
-    const uint32_t key = bound_of<THREADS>(
-        k,
-        [&](auto &&f) {
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j)
-                if (own[j]) f(place_key(own[j]));
-        },
-        sh);
-    bound = key_logit(key);
-    if (threadIdx.x == 0) sh.count = 0;
+    for (int j = 0; j < COUNT; ++j) most = max(most, __builtin_bit_cast(uint32_t, parts[j]) & 0x7fffffffu);
+    most = wave_max(most);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) sh.wave_key[threadIdx.x / kWave] = most;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        if (!own[j]) continue;
-        if (place_key(own[j]) >= key)
-            sh.list[atomicAdd(&sh.count, 1)] = own[j];
-        else
-            dropped(key_logit(place_key(own[j])));
-    }
-    __syncthreads();
-    return sh.count;
+    for (int v = 0; v < THREADS / kWave; ++v) most = max(most, sh.wave_key[v]);
+    if (most >= 0x7f800000u) return NAN;
+    const int up = 40 - (static_cast<int>(most >> 23) - 127);
+    u64 q = 0;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) q += static_cast<u64>(ldexp(static_cast<double>(parts[j]), up));
+    return static_cast<float>(ldexp(static_cast<double>(block_sum(q, sh)), -up));
 }
 
-// Reads the row once and leaves in the list every logit of a bound that at
-// least k logits reach (k <= kList / 4). begin(bound, most), given the first
-// bound (NaN, -inf or +inf: no finite one) and the first slab's largest logit,
-// returns the bound to take: the same, or a higher one where fewer than k
-// will do. Then below(values) is called for every piece, with -inf in place of
-// what was collected or lies past the end, and dropped(value) for a logit that
-// was collected and no longer is. Returns the number collected, in no
+// Reads the row once and leaves in the list every logit at or above `bound`, a
+// bound that at least k logits reach (k <= kList / 4, or the whole row). A
+// piece of which some logit reaches the bound of the moment is put aside as
+// its largest key and its number; when the row has been read, the k-th largest
+// of those keys is the last bound (no piece below it holds one of the first
+// k), and the pieces put aside are read again. Where they become many before
+// the end, the bound is raised early. begin(bound, most), given the first
+// bound (NaN or infinite: no finite one) and, with MOST, the first slab's
+// largest logit, returns the bound to take: the same, or a higher one where
+// fewer than k will do. With SUM, sum(values) is added up over all that is not
+// in the list, which has -inf in its place: total is this thread's share of the
+// stream, extra that of the pieces put aside, whose order among the threads
+// changes from run to run. Returns the number collected, in no
 // particular order, or -1 if they were too many.
-template <bool WANT_MOST, typename T, int THREADS, typename Begin, typename Below, typename Dropped>
-__device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, float &bound, Begin &&begin, Below &&below,
-                       Dropped &&dropped) {
-    constexpr int N = Row<T, THREADS>::N;
+template <bool MOST, bool SUM, typename T, int THREADS, typename Begin, typename Sum>
+__device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, float &bound, float &total, float &extra,
+                       Begin &&begin, Sum &&sum) {
     using R = Row<T, THREADS>;
-    const int slabs = row.slabs(), n = row.n;
+    constexpr int N = R::N, kOwn = kList<THREADS> / THREADS;
+    const int slabs = row.slabs(), n = row.n, tid = threadIdx.x;
     words4 w[kSlab], next[kSlab];
     row.load(0, w);
-    if (threadIdx.x == 0) sh.count = 0;
-    bound = NAN;  // everything reaches it
+    if (tid == 0) sh.count = 0;
     uint32_t most_key = 0;
-    if constexpr (WANT_MOST) {
+    if constexpr (MOST) {
 #pragma unroll
-        for (int u = 0; u < kSlab; ++u) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (R::at(0, u) + i < n) most_key = max(most_key, logit_key(piece_value<T>(w[u], i)));
-        }
+        for (int u = 0; u < kSlab; ++u)
+            if (R::at(0, u) < n) most_key = max(most_key, logit_key(piece_most<T>(w[u])));
         most_key = wave_max(most_key);
-        if ((threadIdx.x & (kWave - 1)) == 0) sh.wave_key[threadIdx.x / kWave] = most_key;
+        if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = most_key;
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < THREADS / kWave; ++v) most_key = max(most_key, sh.wave_key[v]);
     }
-    if ((min(n, R::kSlabLogits) + N - 1) / N >= k) {
-        const uint32_t key = bound_of<THREADS>(
+    const bool few = (min(n, R::kSlabLogits) + N - 1) / N < k;  // pieces: then the row is one slab, bounded logit by logit
+    bound = key_logit(bound_of<THREADS>(
+        min(k, n),
+        [&](auto &&f) {
+            if (few) {
+                row.each([&](float x, int) { f(logit_key(x)); });
+            } else {
+#pragma unroll
+                for (int u = 0; u < kSlab; ++u)
+                    if (R::at(0, u) < n) f(logit_key(piece_most<T>(w[u])));
+            }
+        },
+        sh));
+    bound = begin(bound, key_logit(most_key));
+    total = extra = 0.f;
+
+    // the pieces put aside, this thread's share of them, are summed or read
+    // again: those that reach the bound into the list
+    u64 own[kOwn];
+    int aside = 0;
+    auto take_own = [&] {
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) own[j] = j * THREADS + tid < aside ? sh.list[j * THREADS + tid] : 0;
+    };
+    auto own_bound = [&] {
+        return bound_of<THREADS>(
             k,
             [&](auto &&f) {
 #pragma unroll
-                for (int u = 0; u < kSlab; ++u) {
-                    if (R::at(0, u) < n) {
-                        float most = piece_value<T>(w[u], 0);
-#pragma unroll
-                        for (int i = 1; i < N; ++i) most = nan_max(most, piece_value<T>(w[u], i));
-                        f(logit_key(most));
-                    }
-                }
+                for (int j = 0; j < kOwn; ++j)
+                    if (own[j]) f(place_key(own[j]));
             },
             sh);
-        bound = key_logit(key);
-    }
-    bound = begin(bound, key_logit(most_key));
+    };
+    auto read_again = [&](u64 entry, float (&y)[N]) {
+        const int at = static_cast<int>(static_cast<uint32_t>(entry)) * N;
+        const words4 p = load_piece_to(row.x, at, n);
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = piece_value<T>(p, i);
+        return at;
+    };
+
     __syncthreads();
     for (int slab = 0; slab < slabs; ++slab) {
         if (slab + 1 < slabs) row.load(slab + 1, next);
 #pragma unroll
         for (int u = 0; u < kSlab; ++u) {
-            float y[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) y[i] = piece_value<T>(w[u], i);
-            float most = y[0];
-#pragma unroll
-            for (int i = 1; i < N; ++i) most = nan_max(most, y[i]);
-            if (!(most < bound)) {
-                const int at = R::at(slab, u);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (!(y[i] < bound) && at + i < n) {
-                        const int slot = atomicAdd(&sh.count, 1);
-                        if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(y[i]), at + i);
-                        y[i] = -INFINITY;
-                    }
-                }
+            const float most = piece_most<T>(w[u]);
+            const int at = R::at(slab, u);
+            const bool reaches = !(most < bound) && at < n;
+            if (reaches) {
+                const int slot = atomicAdd(&sh.count, 1);
+                if (slot < kList<THREADS>) sh.list[slot] = static_cast<u64>(logit_key(most)) << 32 | static_cast<uint32_t>(at / N);
             }
-            below(y);
+            if constexpr (SUM) {
+                float y[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = piece_value<T>(w[u], i);
+                const float part = sum(y);
+                total += reaches ? 0.f : part;
+            }
         }
         if (slab + 1 < slabs) {
             __syncthreads();
-            const int count = sh.count;
-            if (count > kList<THREADS>) return -1;
-            if (count > kList<THREADS> / 2) {
-                shrink_list(count, k, bound, dropped, sh);
-            } else {
+            aside = sh.count;
+            if (aside > kList<THREADS>) return -1;
+            __syncthreads();
+            if (aside > kList<THREADS> / 2) {
+                take_own();
+                const uint32_t key = own_bound();
+                bound = key_logit(key);
+                if (tid == 0) sh.count = 0;
+                __syncthreads();
+                float parts[kOwn];
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) {
+                    parts[j] = 0.f;
+                    if (!own[j]) continue;
+                    if (place_key(own[j]) >= key) {
+                        sh.list[atomicAdd(&sh.count, 1)] = own[j];
+                    } else if constexpr (SUM) {
+                        float y[N];
+                        read_again(own[j], y);
+                        parts[j] = sum(y);
+                    }
+                }
+                if constexpr (SUM) extra += sum_in_any_order(parts, sh);
                 __syncthreads();
             }
 #pragma unroll
@@ -432,10 +469,33 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
         }
     }
     __syncthreads();
-    int count = sh.count;
-    if (count > kList<THREADS>) return -1;
-    if (count > 2 * k && count > 256) count = shrink_list(count, k, bound, dropped, sh);
-    return count;
+    aside = sh.count;
+    if (aside > kList<THREADS>) return -1;
+    take_own();
+    if (!few && aside > k) bound = key_logit(own_bound());
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    float parts[kOwn];
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        parts[j] = 0.f;
+        if (!own[j]) continue;
+        float y[N];
+        const int at = read_again(own[j], y);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (!(y[i] < bound) && at + i < n) {
+                const int slot = atomicAdd(&sh.count, 1);
+                if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(y[i]), at + i);
+                y[i] = -INFINITY;
+            }
+        }
+        if constexpr (SUM) parts[j] = sum(y);
+    }
+    if constexpr (SUM) extra += sum_in_any_order(parts, sh);
+    __syncthreads();
+    return sh.count <= kList<THREADS> ? sh.count : -1;
 }
 
 struct TopKernelArgs {
@@ -449,7 +509,7 @@ struct TopKernelArgs {
 };
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void top_logits_kernel(TopKernelArgs a) {
+__global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a) {
     constexpr int N = Row<T, THREADS>::N;
     __shared__ Shared<THREADS> sh;
     const int tid = threadIdx.x;
@@ -460,19 +520,20 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(TopKernelArgs a) {
     // The others' sum, in units of 2^(c bound): all of them are below the bound,
     // so nothing overflows, and only a rest far below it could be lost to
     // underflow.
-    float bound, first_bound = 0.f, offset = 0.f, sum = 0.f;
-    const int n = collect<false>(
-        row, a.k, sh, bound,
+    float bound, first_bound = 0.f, offset = 0.f, sum, extra;
+    const int n = collect<false, true>(
+        row, a.k, sh, bound, sum, extra,
         [&](float b, float) {
             first_bound = fabsf(b) < 1e30f ? b : 0.f;
             offset = first_bound * c;
             return b;
         },
         [&](const float (&y)[N]) {
+            float part = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum += fast_exp2(fmaf(y[i], c, -offset));
-        },
-        [&](float x) { sum += fast_exp2(fmaf(x, c, -offset)); });
+            for (int i = 0; i < N; ++i) part += fast_exp2(fmaf(y[i], c, -offset));
+            return part;
+        });
     u64 cut = 0;
     ExpSum rest;
     if (n < 0) {
@@ -499,7 +560,7 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(TopKernelArgs a) {
     sum = wave_sum(sum);
     if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = __builtin_bit_cast(uint32_t, sum);
     __syncthreads();
-    sum = 0.f;
+    sum = extra;
 #pragma unroll
     for (int w = 0; w < THREADS / kWave; ++w) {
         const uint32_t u = sh.wave_key[w];
@@ -551,6 +612,9 @@ struct Weights {
     float m, inverse;
     __device__ __forceinline__ float of(float x) const { return x == m ? 1.f : fast_exp2((x - m) * inverse); }
     __device__ __forceinline__ u64 fixed(float x) const { return static_cast<u64>(of(x) * kFixed); }
+    // the same where the largest logit is finite: 2^0 is 1
+    __device__ __forceinline__ float of_finite(float x) const { return fast_exp2((x - m) * inverse); }
+    __device__ __forceinline__ u64 fixed_finite(float x) const { return static_cast<u64>(of_finite(x) * kFixed); }
 };
 
 __device__ __forceinline__ u64 limit_of(float top_p, u64 sum) {
@@ -749,13 +813,14 @@ __device__ Drawn draw_from_slabs(const Row<T, THREADS> &row, const u64 *slab_mas
 }
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
-    constexpr int N = Row<T, THREADS>::N, kLanes = kWave - 1;
+__global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) {
+    using R = Row<T, THREADS>;
+    constexpr int N = R::N;
     __shared__ Shared<THREADS> sh;
     __shared__ MassBins mass;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
-    const Row<T, THREADS> row{static_cast<const T *>(a.x) + r * a.stride, a.vocab};
+    const R row{static_cast<const T *>(a.x) + r * a.stride, a.vocab};
     const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
     const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     const float min_p = fminf(a.min_ps ? a.min_ps[r] : a.min_p, 1.f);
@@ -763,6 +828,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
     int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
     if (top_k >= row.n || top_k < 0) top_k = 0;
     const bool greedy = !(temperature > 0.f);
+    // neither 0 nor inf, so that no difference of 0 and none of inf makes a NaN
+    const float inverse = fminf(fmaxf(kLog2e / temperature, 1.17549435e-38f), 3.402823466e38f);
+    const int slabs = row.slabs();
 
     auto answer = [&](int token, float log_prob) {
         if (tid == 0) {
@@ -770,64 +838,66 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
             a.log_probs[r] = log_prob;
         }
     };
-    // neither 0 nor inf, so that no difference of 0 and none of inf makes a NaN
-    const float inverse = fminf(fmaxf(kLog2e / temperature, 1.17549435e-38f), 3.402823466e38f);
-    const int want = greedy ? 1 : top_k > 0 && top_k <= kList<THREADS> / 4 ? top_k : min(min(kGuess, kList<THREADS> / 4), row.n);
-    float bound;
-    int n = collect<true>(
-        row, want, sh, bound,
-        [&](float b, float most) {
-            // what has no weight beside the largest so far is left out: rows of
-            // which a mask leaves little are collected whole
-            const float none = greedy ? most : most - 41.f / inverse;
-            if (!(none > -3.402823466e38f)) return b == b ? fmaxf(b, -3.402823466e38f) : -3.402823466e38f;
-            return b == b ? fmaxf(b, none) : none;
-        },
-        [](const float (&)[N]) {}, [](float) {});
-    const bool defeated = n < 0;
-    u64 top;
-    if (n == 0) return answer(-1, NAN);  // no logit above -inf
-    if (defeated) {
-        top = find_cut(row, 1, [](float, int) -> u64 { return 1; }, sh);
-        if (place_index(top, row.n) == row.n - 1)  // a cut among equals names no index
-            top = place(place_key(top), find_by_index(row, 0, [&](float x, int) -> u64 { return logit_key(x) == place_key(top); }, sh));
-    } else {
-        sort_list(n, sh);
-        top = sh.list[0];
-    }
-    if (place_key(top) == kKeyNan || place_key(top) == kKeyNegInf) return answer(-1, NAN);
-    if (greedy) return answer(place_index(top, row.n), 0.f);
-    const Weights w{key_logit(place_key(top)), inverse};
     auto finish = [&](const Drawn &d) {
         answer(d.token, logf(static_cast<float>(static_cast<double>(d.weight) / static_cast<double>(d.sum))));
     };
-    if (defeated || top_k > kList<THREADS> / 4 || w.m == INFINITY)
-        return finish(draw_by_search(row, w, top_k, top_p, min_p, u, sh));
 
-    if (top_k > 0) {
-        top_k = min(top_k, n);  // the others have no weight
-        u64 limit = ~0ull;
-        if (top_p < 1.f) {
-            u64 sum = 0;
-            for (int j = tid; j < top_k; j += THREADS) sum += w.fixed(key_logit(place_key(sh.list[j])));
-            limit = limit_of(top_p, block_sum(sum, sh));
+    if (greedy || (top_k > 0 && top_k <= kList<THREADS> / 4)) {
+        float bound, unused, none_aside;
+        int n = collect<true, false>(
+            row, greedy ? 1 : top_k, sh, bound, unused, none_aside,
+            [&](float b, float most) {
+                // what has no weight beside the largest so far is left out: rows of
+                // which a mask leaves little are collected whole
+                const float none = fmaxf(greedy ? most : most - 41.f / inverse, -3.402823466e38f);
+                return b == b ? fmaxf(b, none) : none;
+            },
+            [](const float (&)[N]) { return 0.f; });
+        if (n == 0) return answer(-1, NAN);  // no logit above -inf
+        if (n > 0) {
+            sort_list(n, sh);
+            const u64 top = sh.list[0];
+            const Weights w{key_logit(place_key(top)), inverse};
+            if (place_key(top) == kKeyNan || place_key(top) == kKeyNegInf) return answer(-1, NAN);
+            if (greedy) return answer(place_index(top, row.n), 0.f);
+            if (w.m < INFINITY) {
+                n = min(top_k, n);
+                u64 limit = ~0ull;
+                if (top_p < 1.f) {
+                    u64 sum = 0;
+                    for (int j = tid; j < n; j += THREADS) sum += w.fixed(key_logit(place_key(sh.list[j])));
+                    limit = limit_of(top_p, block_sum(sum, sh));
+                }
+                return finish(draw_from_list(n, limit, w, min_p, u, row.n, sh));
+            }
         }
-        return finish(draw_from_list(top_k, limit, w, min_p, u, row.n, sh));
     }
-    const bool all_listed = n == row.n || (bound == bound && w.fixed(bound) == 0);
-    if (all_listed || (!(top_p < 1.f) && w.of(bound) < min_p)) {  // nothing below the bound can be kept
-        u64 limit = ~0ull;
-        if (top_p < 1.f) {
-            u64 sum = 0;
-            for (int j = tid; j < n; j += THREADS) sum += w.fixed(key_logit(place_key(sh.list[j])));
-            limit = limit_of(top_p, block_sum(sum, sh));
+
+    // the largest logit
+    uint32_t top = 0;
+    {
+        float most = -INFINITY;
+        for (int s = 0; s < slabs; ++s) {
+            words4 w[kSlab];
+            row.load(s, w);
+#pragma unroll
+            for (int p = 0; p < kSlab; ++p) most = nan_max(most, piece_most<T>(w[p]));
         }
-        return finish(draw_from_list(n, limit, w, min_p, u, row.n, sh));
+        top = wave_max(logit_key(most));
+        __syncthreads();
+        if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < THREADS / kWave; ++v) top = max(top, sh.wave_key[v]);
     }
-    const int slabs = row.slabs();
+    if (top == kKeyNan || top == kKeyNegInf) return answer(-1, NAN);
+    if (greedy) return answer(find_by_index(row, 0, [&](float x, int) -> u64 { return logit_key(x) == top; }, sh), 0.f);
+    const Weights w{key_logit(top), inverse};
+    if (top_k > 0 || w.m == INFINITY) return finish(draw_by_search(row, w, top_k, top_p, min_p, u, sh));
+
     for (int s = tid; s < kMaxSlabs; s += THREADS) mass.slab[s] = 0;
     if (!(top_p < 1.f)) {
-        auto kept = [&](float x, int) -> u64 { return w.of(x) >= min_p ? w.fixed(x) : 0; };
+        auto kept = [&](float x, int) -> u64 { return w.of_finite(x) >= min_p ? w.fixed_finite(x) : 0; };
         __syncthreads();
         for (int s = 0; s < slabs; ++s) {
             u64 sum = 0;
@@ -836,7 +906,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
                 for (int i = 0; i < N; ++i) sum += kept(y[i], 0);
             });
             sum = wave_add(sum);
-            if ((tid & kLanes) == 0) atomicAdd(&mass.slab[s], sum);
+            if ((tid & (kWave - 1)) == 0) atomicAdd(&mass.slab[s], sum);
         }
         __syncthreads();
         return finish(draw_from_slabs(row, mass.slab, u, kept, sh));
@@ -849,7 +919,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
         row.pieces(s, [&](const float (&y)[N], int) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const u64 f = w.fixed(y[i]);
+                const u64 f = w.fixed_finite(y[i]);
                 if (f) atomicAdd(&mass.bins[mass_bin(y[i], w)], f);
             }
         });
@@ -861,13 +931,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
     for (int j = 0; j < kOwnBins; ++j) own += mass.bins[tid * kOwnBins + j];
     u64 before = block_scan(own, total, sh);
     const u64 limit = limit_of(top_p, total);
-    own = 0;
-    for (int j = tid; j < n; j += THREADS) own += w.fixed(key_logit(place_key(sh.list[j])));
-    if (block_sum(own, sh) >= limit) return finish(draw_from_list(n, limit, w, min_p, u, row.n, sh));
 
-    // the prefix ends in a bin past the list: what is in the bins before is
-    // kept, the bin's own logits are sorted
-    __syncthreads();
+    // the prefix ends in one of the bins: what is in the bins before is kept,
+    // the bin's own logits are sorted
     for (int j = 0; j < kOwnBins; ++j) {
         const u64 in_bin = mass.bins[tid * kOwnBins + j];
         if (before < limit && limit <= before + in_bin) {
@@ -880,41 +946,49 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
     __syncthreads();
     const int cut_bin = static_cast<int>(sh.pick[0]);
     const u64 above = sh.pick[1];
+    // below this no logit is in the bins kept (a margin of two bins)
+    const float least = w.m - (static_cast<float>(cut_bin) + 3.f) * (40.f / kMassBins) / w.inverse;
     for (int s = 0; s < slabs; ++s) {
         u64 sum = 0;
-        row.pieces(s, [&](const float (&y)[N], int at) {
+        words4 p[kSlab];
+        row.load(s, p);
+#pragma unroll
+        for (int k = 0; k < kSlab; ++k) {
+            if (piece_most<T>(p[k]) < least) continue;
+            const int at = R::at(s, k);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const u64 f = w.fixed(y[i]);
+                const float x = piece_value<T>(p[k], i);
+                const u64 f = w.fixed_finite(x);
                 if (!f) continue;
-                const int b = mass_bin(y[i], w);
+                const int b = mass_bin(x, w);
                 if (b < cut_bin) {
-                    if (w.of(y[i]) >= min_p) sum += f;
+                    if (w.of_finite(x) >= min_p) sum += f;
                 } else if (b == cut_bin) {
                     const int slot = atomicAdd(&sh.count, 1);
-                    if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(y[i]), at + i);
+                    if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(x), at + i);
                 }
             }
-        });
+        }
         sum = wave_add(sum);
-        if ((tid & kLanes) == 0) atomicAdd(&mass.slab[s], sum);
+        if ((tid & (kWave - 1)) == 0) atomicAdd(&mass.slab[s], sum);
     }
     __syncthreads();
-    n = sh.count;
+    const int n = sh.count;
     if (n > kList<THREADS>) return finish(draw_by_search(row, w, top_k, top_p, min_p, u, sh));
     sort_list(n, sh);
     const int per = (n + THREADS - 1) / THREADS, from = tid * per;
     own = 0;
     for (int j = 0; j < per; ++j)
-        if (from + j < n) own += w.fixed(key_logit(place_key(sh.list[from + j])));
+        if (from + j < n) own += w.fixed_finite(key_logit(place_key(sh.list[from + j])));
     before = above + block_scan(own, total, sh);
     __syncthreads();
     for (int j = 0; j < per; ++j) {
         if (from + j < n && before < limit) {
             const u64 p = sh.list[from + j];
             const float x = key_logit(place_key(p));
-            const u64 f = w.fixed(x);
-            if (w.of(x) >= min_p) atomicAdd(&mass.slab[place_index(p, row.n) / Row<T, THREADS>::kSlabLogits], f);
+            const u64 f = w.fixed_finite(x);
+            if (w.of_finite(x) >= min_p) atomicAdd(&mass.slab[place_index(p, row.n) / R::kSlabLogits], f);
             before += f;
             if (before >= limit) sh.pick[0] = p;  // the last one kept
         }
@@ -924,7 +998,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleKernelArgs a) {
     __syncthreads();
     finish(draw_from_slabs(
         row, mass.slab, u,
-        [&](float x, int i) -> u64 { return place(logit_key(x), i) >= cut && w.of(x) >= min_p ? w.fixed(x) : 0; }, sh));
+        [&](float x, int i) -> u64 {
+            return place(logit_key(x), i) >= cut && w.of_finite(x) >= min_p ? w.fixed_finite(x) : 0;
+        },
+        sh));
 }
 
 // Threads for a row: its pieces fill a slab or a few, and no row has more
