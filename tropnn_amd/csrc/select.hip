@@ -25,8 +25,11 @@ namespace {
 
 constexpr int kBins = 256;
 constexpr int kSlab = 8;        // pieces of a thread that are in flight together
+constexpr int kKeyBins = 2048;  // of keys, by their distance from the largest
+constexpr int kKeyShift = 15;   // 2^15 keys a bin, 256 bins an octave
 constexpr int kMassBins = 2048; // of a row's weights, by exponent
-constexpr int kMaxSlabs = 64;
+constexpr int kRanked = 1024;   // logits sorted by counting
+constexpr int kMaxChunks = 512; // a wave's share of a slab, in the widest row
 constexpr float kFixed = 1099511627776.f;  // 2^40: sampling weights are multiples of 2^-40
 
 using u64 = unsigned long long;
@@ -63,9 +66,12 @@ struct Shared {
     union {
         u64 bins[kBins];
         uint32_t counts[kBins];
+        uint32_t key_counts[kKeyBins];
+        uint32_t ranks[kRanked];
+        u64 mass[kMassBins];
     };
     u64 wave[kWaves < 2 ? 2 : kWaves];
-    u64 pick[2];
+    u64 pick[3];
     float2 wave_rest[kWaves];
     uint32_t wave_key[kWaves];
     int count;
@@ -82,9 +88,12 @@ struct Row {
 
     __device__ __forceinline__ int slabs() const { return (n + kSlabLogits - 1) / kSlabLogits; }
 
-    // The first logit of piece u of this thread in a slab.
+    // The first logit of piece u of this thread in a slab. A wave's pieces of
+    // a slab are one chunk of the row.
+    static constexpr int kChunk = kWave * kSlab * N;
+    static __device__ __forceinline__ int chunk(int slab) { return slab * (THREADS / kWave) + static_cast<int>(threadIdx.x) / kWave; }
     static __device__ __forceinline__ int at(int slab, int u) {
-        return slab * kSlabLogits + (u * THREADS + static_cast<int>(threadIdx.x)) * N;
+        return chunk(slab) * kChunk + (u * kWave + (static_cast<int>(threadIdx.x) & (kWave - 1))) * N;
     }
     // Logits past the row's end are -inf.
     __device__ __forceinline__ void load(int slab, words4 (&w)[kSlab]) const {
@@ -102,20 +111,6 @@ struct Row {
             }
         }
     }
-    // f(values, index of the first) for every piece; values past the end are
-    // -inf.
-    template <typename F>
-    __device__ __forceinline__ void pieces(int slab, F &&f) const {
-        words4 w[kSlab];
-        load(slab, w);
-#pragma unroll
-        for (int u = 0; u < kSlab; ++u) {
-            float y[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) y[i] = piece_value<T>(w[u], i);
-            f(y, at(slab, u));
-        }
-    }
     // f(value, index) for every logit
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {
@@ -128,14 +123,32 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ u64 wave_scan(u64 v) {  // the lanes' sum up to and with this one
-    const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const u64 o = __shfl_up(v, d, kWave);
-        if (lane >= d) v += o;
-    }
+// Lane l gets lane l - n's value within its row of 16 (CTRL row_shr:n), or the
+// last of the row or the two rows before it (row_bcast), else 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_from(u64 v) {
+    const uint32_t low = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v)), high = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v >> 32));
+    return static_cast<u64>(high) << 32 | low;
+}
+
+// The lanes' sum up to and with this one.
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v += dpp_from<0x111, 0xF>(v);
+    v += dpp_from<0x112, 0xF>(v);
+    v += dpp_from<0x114, 0xF>(v);
+    v += dpp_from<0x118, 0xF>(v);
+    v += dpp_from<0x142, 0xA>(v);
+    v += dpp_from<0x143, 0xC>(v);
     return v;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), kWave - 1)); }
+__device__ __forceinline__ u64 last_lane(u64 v) {
+    return static_cast<u64>(last_lane(static_cast<uint32_t>(v >> 32))) << 32 | last_lane(static_cast<uint32_t>(v));
 }
 
 // The sum of the threads' values before this one's, and of all.
@@ -162,6 +175,17 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared<THREADS> &sh) {
     u64 total;
     block_scan(v, total, sh);
     return total;
+}
+
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, Shared<THREADS> &sh) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) sh.wave_key[threadIdx.x / kWave] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / kWave; ++w) v = max(v, sh.wave_key[w]);
+    return v;
 }
 
 // ---- the exact search, for any row ----
@@ -277,21 +301,80 @@ __device__ void sort_down(u64 *v, int n) {
 
 __device__ __forceinline__ int slots_for(int n) { return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)); }
 
-// Sorts the n collected logits.
+// Sorts the first n numbers of the list (all different), largest first. A
+// number's place is the count of larger ones; the threads share the counting.
+// n^2 / THREADS comparisons against broadcast reads beat the sorting network's
+// chain of LDS round trips (80 numbers, 512 threads: 5 us with the network)
+// until they are many.
 template <int THREADS>
 __device__ void sort_list(int n, Shared<THREADS> &sh) {
-    const int slots = slots_for(n);
+    const int tid = threadIdx.x, slots = slots_for(max(n, kWave));
     __syncthreads();
-    for (int i = n + static_cast<int>(threadIdx.x); i < slots; i += THREADS) sh.list[i] = 0;
-    sort_down<THREADS>(sh.list, slots);
+    if (n > kRanked || slots > THREADS) {
+        const int padded = slots_for(n);
+        for (int i = n + tid; i < padded; i += THREADS) sh.list[i] = 0;
+        sort_down<THREADS>(sh.list, padded);
+        return;
+    }
+    const int i = tid & (slots - 1), part = tid / slots, parts = THREADS / slots;
+    const int per = (n + parts - 1) / parts, to = min(n, (part + 1) * per);
+    const u64 v = i < n ? sh.list[i] : 0;
+    if (part == 0) sh.ranks[i] = 0;
+    uint32_t rank = 0;
+#pragma unroll 4
+    for (int j = part * per; j < to; ++j) rank += sh.list[j] > v;
+    __syncthreads();
+    if (i < n && rank) atomicAdd(&sh.ranks[i], rank);
+    __syncthreads();
+    if (part == 0 && i < n) sh.list[min(static_cast<int>(sh.ranks[i]), n - 1)] = v;
+    __syncthreads();
 }
 
-// The largest multiple of 2^16 that at least k of the keys reach; keys(f)
-// calls f for this thread's keys, and there are at least k in all.
+// A key that at least k of the given ones reach, and few more; keys(f) calls f
+// for this thread's, and there are at least k in all. The keys are counted by
+// their distance from the largest, in bins of 2^15: of a positive largest they
+// resolve 2^-8 of it over eight octaves, as finely as bf16, and spread even keys
+// of one exponent over many bins (the threads' additions to one bin go one by
+// one). Where the k-th is farther, digit by digit: 16 bits of it.
 template <int THREADS, typename K>
 __device__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
+    constexpr int kOwn = kKeyBins / THREADS;
     const int tid = threadIdx.x;
-    uint32_t bound = 0, need = static_cast<uint32_t>(k);
+    const uint32_t wanted = static_cast<uint32_t>(k);
+    uint32_t most = 0;
+    keys([&](uint32_t key) { most = max(most, key); });
+    most = wave_max(most);
+    __syncthreads();
+    if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = most;
+    for (int b = tid; b < kKeyBins; b += THREADS) sh.key_counts[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < THREADS / kWave; ++v) most = max(most, sh.wave_key[v]);
+    keys([&](uint32_t key) { atomicAdd(&sh.key_counts[min((most - key) >> kKeyShift, static_cast<uint32_t>(kKeyBins - 1))], 1u); });
+    __syncthreads();
+    uint32_t own = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) own += sh.key_counts[tid * kOwn + j];
+    const uint32_t upto = wave_scan(own);
+    if ((tid & (kWave - 1)) == kWave - 1) sh.wave_key[tid / kWave] = upto;
+    __syncthreads();
+    uint32_t before = upto - own;
+#pragma unroll
+    for (int v = 0; v < THREADS / kWave; ++v) before += v < tid / kWave ? sh.wave_key[v] : 0;
+    if (before < wanted && wanted <= before + own) {
+        int bin = tid * kOwn;
+        while (before + sh.key_counts[bin] < wanted) before += sh.key_counts[bin++];
+        sh.bound = static_cast<uint32_t>(bin);
+    }
+    __syncthreads();
+    const uint32_t bin = sh.bound;
+    // a bin holds the keys down to most - (bin + 1) * 2^15 + 1
+    if (bin < kKeyBins - 1) {
+        const uint32_t span = ((bin + 1) << kKeyShift) - 1;
+        return most > span ? most - span : 0;
+    }
+
+    uint32_t bound = 0, need = wanted;
 #pragma unroll 1
     for (int shift = 24; shift >= 16; shift -= 8) {
         __syncthreads();
@@ -303,13 +386,13 @@ __device__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
         __syncthreads();
         if (tid < kWave) {
             const int top = kBins - 1 - 4 * tid;
-            const u64 own = sh.counts[top] + sh.counts[top - 1] + sh.counts[top - 2] + sh.counts[top - 3];
-            u64 before = wave_scan(own) - own;
-            if (before < need && need <= before + own) {
+            const uint32_t four = sh.counts[top] + sh.counts[top - 1] + sh.counts[top - 2] + sh.counts[top - 3];
+            uint32_t above = wave_scan(four) - four;
+            if (above < need && need <= above + four) {
                 int digit = top;
-                while (before + sh.counts[digit] < need) before += sh.counts[digit--];
+                while (above + sh.counts[digit] < need) above += sh.counts[digit--];
                 sh.bound = bound | static_cast<uint32_t>(digit) << shift;
-                sh.pick[1] = need - before;
+                sh.pick[1] = need - above;
             }
         }
         __syncthreads();
@@ -327,12 +410,7 @@ __device__ float sum_in_any_order(const float (&parts)[COUNT], Shared<THREADS> &
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < COUNT; ++j) most = max(most, __builtin_bit_cast(uint32_t, parts[j]) & 0x7fffffffu);
-    most = wave_max(most);
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) sh.wave_key[threadIdx.x / kWave] = most;
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < THREADS / kWave; ++v) most = max(most, sh.wave_key[v]);
+    most = block_max(most, sh);
     if (most >= 0x7f800000u) return NAN;
     const int up = 40 - (static_cast<int>(most >> 23) - 127);
     u64 q = 0;
@@ -369,11 +447,7 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
 #pragma unroll
         for (int u = 0; u < kSlab; ++u)
             if (R::at(0, u) < n) most_key = max(most_key, logit_key(piece_most<T>(w[u])));
-        most_key = wave_max(most_key);
-        if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = most_key;
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < THREADS / kWave; ++v) most_key = max(most_key, sh.wave_key[v]);
+        most_key = block_max(most_key, sh);
     }
     const bool few = (min(n, R::kSlabLogits) + N - 1) / N < k;  // pieces: then the row is one slab, bounded logit by logit
     bound = key_logit(bound_of<THREADS>(
@@ -399,15 +473,16 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
 #pragma unroll
         for (int j = 0; j < kOwn; ++j) own[j] = j * THREADS + tid < aside ? sh.list[j * THREADS + tid] : 0;
     };
-    auto own_bound = [&] {
-        return bound_of<THREADS>(
+    auto raise = [&] {
+        const float next = key_logit(bound_of<THREADS>(
             k,
             [&](auto &&f) {
 #pragma unroll
                 for (int j = 0; j < kOwn; ++j)
                     if (own[j]) f(place_key(own[j]));
             },
-            sh);
+            sh));
+        if (!(next < bound)) bound = next;
     };
     auto read_again = [&](u64 entry, float (&y)[N]) {
         const int at = static_cast<int>(static_cast<uint32_t>(entry)) * N;
@@ -444,8 +519,7 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
             __syncthreads();
             if (aside > kList<THREADS> / 2) {
                 take_own();
-                const uint32_t key = own_bound();
-                bound = key_logit(key);
+                raise();
                 if (tid == 0) sh.count = 0;
                 __syncthreads();
                 float parts[kOwn];
@@ -453,7 +527,7 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
                 for (int j = 0; j < kOwn; ++j) {
                     parts[j] = 0.f;
                     if (!own[j]) continue;
-                    if (place_key(own[j]) >= key) {
+                    if (!(key_logit(place_key(own[j])) < bound)) {
                         sh.list[atomicAdd(&sh.count, 1)] = own[j];
                     } else if constexpr (SUM) {
                         float y[N];
@@ -472,7 +546,7 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
     aside = sh.count;
     if (aside > kList<THREADS>) return -1;
     take_own();
-    if (!few && aside > k) bound = key_logit(own_bound());
+    if (!few && aside > k) raise();
     __syncthreads();
     if (tid == 0) sh.count = 0;
     __syncthreads();
@@ -610,11 +684,19 @@ struct SampleKernelArgs {
 // What a row's sampling weights need.
 struct Weights {
     float m, inverse;
+    // 1 for the largest, an infinite one too
     __device__ __forceinline__ float of(float x) const { return x == m ? 1.f : fast_exp2((x - m) * inverse); }
-    __device__ __forceinline__ u64 fixed(float x) const { return static_cast<u64>(of(x) * kFixed); }
-    // the same where the largest logit is finite: 2^0 is 1
-    __device__ __forceinline__ float of_finite(float x) const { return fast_exp2((x - m) * inverse); }
-    __device__ __forceinline__ u64 fixed_finite(float x) const { return static_cast<u64>(of_finite(x) * kFixed); }
+    __device__ __forceinline__ u64 fixed(float x) const { return whole(of(x)); }
+    // the exponent, where the largest logit is finite
+    __device__ __forceinline__ float exponent(float x) const { return (x - m) * inverse; }
+    // floor(2^40 e): exact products with powers of two, so the two halves are
+    static __device__ __forceinline__ u64 whole(float e) {
+        const float high = truncf(e * 256.f);
+        const uint32_t low = static_cast<uint32_t>(fmaf(e, kFixed, high * -4294967296.f));
+        return static_cast<u64>(static_cast<uint32_t>(high)) << 32 | low;
+    }
+    // the same as an f64: a thread's sum over a slab stays below 2^53, so it is exact
+    static __device__ __forceinline__ double whole_f64(float e) { return static_cast<double>(truncf(e * kFixed)); }
 };
 
 __device__ __forceinline__ u64 limit_of(float top_p, u64 sum) {
@@ -656,155 +738,117 @@ __device__ Drawn draw_by_search(const Row<T, THREADS> &row, const Weights &w, in
     return d;
 }
 
-// Draws among the first `n` of the sorted list, which hold everything that
-// top_k leaves or that can be kept; `limit` of the mass is top_p's.
+// Draws among the first n of the sorted list, which are all that top_k leaves
+// (but for logits without weight). The first wave has the list's sums.
 template <int THREADS>
-__device__ Drawn draw_from_list(int n, u64 limit, const Weights &w, float min_p, float u, int vocab, Shared<THREADS> &sh) {
-    constexpr int kOwn = kList<THREADS> / THREADS;
-    // the kept logits are the first ones of the list: how many, and their sum
-    const int per = (n + THREADS - 1) / THREADS, from = static_cast<int>(threadIdx.x) * per;
-    u64 own = 0;
-    for (int j = 0; j < per; ++j)
-        if (from + j < n) own += w.fixed(key_logit(place_key(sh.list[from + j])));
-    u64 total;
-    u64 before = block_scan(own, total, sh);
-    u64 sum = 0;
-    int kept = 0;
-    for (int j = 0; j < per; ++j) {
-        if (from + j < n) {
-            const float x = key_logit(place_key(sh.list[from + j]));
-            const u64 f = w.fixed(x);
-            if (before < limit && w.of(x) >= min_p) {
+__device__ Drawn draw_from_list(int n, const Weights &w, float top_p, float min_p, float u, int vocab, Shared<THREADS> &sh) {
+    const int tid = threadIdx.x;
+    if (tid < kWave) {
+        const int per = (n + kWave - 1) / kWave, from = tid * per, to = min(n, from + per);
+        u64 own = 0;
+        for (int j = from; j < to; ++j) own += w.fixed(key_logit(place_key(sh.list[j])));
+        const u64 upto = wave_scan(own), total = last_lane(upto);
+        const u64 limit = top_p < 1.f ? limit_of(top_p, total) : ~0ull;
+        u64 before = upto - own, sum = 0;
+        uint32_t kept = 0;
+        for (int j = from; j < to; ++j) {
+            const float e = w.of(key_logit(place_key(sh.list[j])));
+            const u64 f = Weights::whole(e);
+            if (before < limit && e >= min_p) {
                 ++kept;
                 sum += f;
             }
             before += f;
         }
-    }
-    Drawn d;
-    d.sum = block_sum(sum, sh);
-    kept = static_cast<int>(block_sum(static_cast<u64>(kept), sh));
-    // by index: halves swapped, the larger complement of the index is first
-    u64 turned[kOwn];
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        const int i = j * THREADS + static_cast<int>(threadIdx.x);
-        turned[j] = i < kept ? sh.list[i] << 32 | sh.list[i] >> 32 : 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        const int i = j * THREADS + static_cast<int>(threadIdx.x);
-        if (i < kept) sh.list[i] = turned[j];
-    }
-    sort_list(kept, sh);
-    const u64 target = target_of(u, d.sum);
-    const int each = (kept + THREADS - 1) / THREADS, first = static_cast<int>(threadIdx.x) * each;
-    own = 0;
-    for (int j = 0; j < each; ++j)
-        if (first + j < kept) own += w.fixed(key_logit(static_cast<uint32_t>(sh.list[first + j])));
-    before = block_scan(own, total, sh);
-    if (before <= target && target < before + own) {
-        int j = first;
-        u64 f = w.fixed(key_logit(static_cast<uint32_t>(sh.list[j])));
-        while (target >= before + f) {
-            before += f;
-            f = w.fixed(key_logit(static_cast<uint32_t>(sh.list[++j])));
+        // the kept logits are the first ones of the list
+        sum = last_lane(wave_scan(sum));
+        kept = last_lane(wave_scan(kept));
+        if (tid == 0) {
+            sh.pick[0] = sum;
+            sh.pick[1] = kept;
         }
-        sh.pick[0] = sh.list[j] >> 32;
-        sh.pick[1] = f;
     }
     __syncthreads();
-    d.token = place_index(sh.pick[0], vocab);
+    Drawn d;
+    d.sum = sh.pick[0];
+    const int kept = static_cast<int>(sh.pick[1]);
+    if (kept == 1) {
+        d.token = place_index(sh.list[0], vocab);
+        d.weight = d.sum;
+        return d;
+    }
+    // by index: halves swapped, the larger complement of the index is first
+    for (int i = tid; i < kept; i += THREADS) sh.list[i] = sh.list[i] << 32 | sh.list[i] >> 32;
+    sort_list(kept, sh);
+    if (tid < kWave) {
+        const u64 target = target_of(u, d.sum);
+        const int per = (kept + kWave - 1) / kWave, from = tid * per, to = min(kept, from + per);
+        u64 own = 0;
+        for (int j = from; j < to; ++j) own += w.fixed(key_logit(static_cast<uint32_t>(sh.list[j])));
+        u64 before = wave_scan(own) - own;
+        if (before <= target && target < before + own) {
+            int j = from;
+            u64 f = w.fixed(key_logit(static_cast<uint32_t>(sh.list[j])));
+            while (j + 1 < to && target >= before + f) {
+                before += f;
+                f = w.fixed(key_logit(static_cast<uint32_t>(sh.list[++j])));
+            }
+            sh.pick[1] = f;
+            sh.pick[2] = sh.list[j] >> 32;
+        }
+    }
+    __syncthreads();
     d.weight = sh.pick[1];
+    d.token = place_index(sh.pick[2], vocab);
     return d;
 }
 
-// The weights of a row's logits by exponent, largest first.
-struct MassBins {
-    u64 bins[kMassBins];
-    u64 slab[kMaxSlabs];
-};
+// The bin of an exponent y <= 0, as a number to compare whole ones with:
+// monotone in the logit, 0 for the largest, below kMassBins for a weight that
+// is not 0.
+__device__ __forceinline__ float mass_bin(float y) { return y * (-kMassBins / 41.f); }
 
-// The bin of a weight 2^-a: a / 40 of them all, monotone in the logit.
-__device__ __forceinline__ int mass_bin(float x, const Weights &w) {
-    const float a = (w.m - x) * w.inverse;
-    return static_cast<int>(fminf(a * (kMassBins / 40.f), static_cast<float>(kMassBins - 1)));
-}
-
-// Draws from all logits of which mass(value, index) is not 0, given the mass
-// of every slab.
+// Draws from all logits of which mass(value, index) is not 0, given its sum
+// over every chunk.
 template <typename T, int THREADS, typename M>
-__device__ Drawn draw_from_slabs(const Row<T, THREADS> &row, const u64 *slab_mass, float u, M &&mass,
-                                 Shared<THREADS> &sh) {
-    constexpr int N = Row<T, THREADS>::N, kWaves = THREADS / kWave;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int slabs = row.slabs();
-    Drawn d;
-    d.sum = 0;
-    for (int s = 0; s < slabs; ++s) d.sum += slab_mass[s];
-    u64 target = target_of(u, d.sum);
-    int slab = 0;
-    while (slab + 1 < slabs && target >= slab_mass[slab]) target -= slab_mass[slab++];
-    // in that slab: which piece of which wave, by the pieces' order
-    words4 p[kSlab];
-    row.load(slab, p);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSlab; ++k) {
+__device__ Drawn draw_from_chunks(const Row<T, THREADS> &row, const u64 *chunks, float u, M &&mass, Shared<THREADS> &sh) {
+    using R = Row<T, THREADS>;
+    constexpr int kEach = R::kChunk / THREADS;
+    const int tid = threadIdx.x;
+    if (tid < kWave) {
+        const int n = (row.n + R::kChunk - 1) / R::kChunk, per = (n + kWave - 1) / kWave;
+        const int from = tid * per, to = min(n, from + per);
         u64 own = 0;
-        const int at = Row<T, THREADS>::at(slab, k);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (at + i < row.n) own += mass(piece_value<T>(p[k], i), at + i);
-        own = wave_add(own);
-        if (lane == 0) sh.list[k * kWaves + wave] = own;
+        for (int c = from; c < to; ++c) own += chunks[c];
+        const u64 upto = wave_scan(own), sum = last_lane(upto), target = target_of(u, sum);
+        u64 before = upto - own;
+        if (before <= target && target < upto) {
+            int c = from;
+            while (c + 1 < to && target >= before + chunks[c]) before += chunks[c++];
+            sh.pick[0] = static_cast<u64>(c);
+            sh.pick[1] = target - before;
+        }
+        if (tid == 0) sh.pick[2] = sum;
     }
     __syncthreads();
-    constexpr int kSums = kSlab * kWaves, kEach = (kSums + kWave - 1) / kWave;
-    u64 mine[kEach], all = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        mine[j] = lane * kEach + j < kSums ? sh.list[lane * kEach + j] : 0;
-        all += mine[j];
-    }
-    u64 upto = wave_scan(all) - all;
-    int which = -1;
-    u64 less = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        if (upto <= target && target < upto + mine[j]) {
-            which = lane * kEach + j;
-            less = upto;
+    Drawn d;
+    d.sum = sh.pick[2];
+    const u64 target = sh.pick[1];
+    const int from = static_cast<int>(sh.pick[0]) * R::kChunk + tid * kEach;
+    u64 own = 0, total;
+    for (int i = 0; i < kEach; ++i)
+        if (from + i < row.n) own += mass(static_cast<float>(row.x[from + i]), from + i);
+    u64 before = block_scan(own, total, sh);
+    if (before <= target && target < before + own) {
+        int i = 0;
+        u64 f = mass(static_cast<float>(row.x[from]), from);
+        while (i + 1 < kEach && from + i + 1 < row.n && target >= before + f) {
+            before += f;
+            ++i;
+            f = mass(static_cast<float>(row.x[from + i]), from + i);
         }
-        upto += mine[j];
-    }
-    const u64 holders = __ballot(which >= 0);
-    const int holder = holders ? __builtin_ctzll(holders) : 0;
-    which = max(__shfl(which, holder, kWave), 0);
-    target -= __shfl(less, holder, kWave);
-    const int from = slab * Row<T, THREADS>::kSlabLogits + which * kWave * N;
-    if (wave == 0) {
-        const int at = from + lane * N;
-        u64 v[N], own = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[i] = at + i < row.n ? mass(static_cast<float>(row.x[at + i]), at + i) : 0;
-            own += v[i];
-        }
-        u64 before = wave_scan(own) - own;
-        if (before <= target && target < before + own) {
-            int found = -1;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (found < 0 && target < before + v[i]) {
-                    found = at + i;
-                    sh.pick[1] = v[i];
-                }
-                before += v[i];
-            }
-            sh.pick[0] = static_cast<u64>(found);
-        }
+        sh.pick[0] = static_cast<u64>(from + i);
+        sh.pick[1] = f;
     }
     __syncthreads();
     d.token = min(static_cast<int>(sh.pick[0]), row.n - 1);
@@ -817,8 +861,8 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
     using R = Row<T, THREADS>;
     constexpr int N = R::N;
     __shared__ Shared<THREADS> sh;
-    __shared__ MassBins mass;
-    const int tid = threadIdx.x;
+    __shared__ u64 chunks[kMaxChunks];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const int64_t r = blockIdx.x;
     const R row{static_cast<const T *>(a.x) + r * a.stride, a.vocab};
     const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
@@ -844,7 +888,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
 
     if (greedy || (top_k > 0 && top_k <= kList<THREADS> / 4)) {
         float bound, unused, none_aside;
-        int n = collect<true, false>(
+        const int n = collect<true, false>(
             row, greedy ? 1 : top_k, sh, bound, unused, none_aside,
             [&](float b, float most) {
                 // what has no weight beside the largest so far is left out: rows of
@@ -860,82 +904,86 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
             const Weights w{key_logit(place_key(top)), inverse};
             if (place_key(top) == kKeyNan || place_key(top) == kKeyNegInf) return answer(-1, NAN);
             if (greedy) return answer(place_index(top, row.n), 0.f);
-            if (w.m < INFINITY) {
-                n = min(top_k, n);
-                u64 limit = ~0ull;
-                if (top_p < 1.f) {
-                    u64 sum = 0;
-                    for (int j = tid; j < n; j += THREADS) sum += w.fixed(key_logit(place_key(sh.list[j])));
-                    limit = limit_of(top_p, block_sum(sum, sh));
-                }
-                return finish(draw_from_list(n, limit, w, min_p, u, row.n, sh));
-            }
+            if (w.m < INFINITY) return finish(draw_from_list(min(top_k, n), w, top_p, min_p, u, row.n, sh));
         }
     }
 
     // the largest logit
-    uint32_t top = 0;
-    {
-        float most = -INFINITY;
-        for (int s = 0; s < slabs; ++s) {
-            words4 w[kSlab];
-            row.load(s, w);
+    float most = -INFINITY;
+    for (int s = 0; s < slabs; ++s) {
+        words4 p[kSlab];
+        row.load(s, p);
 #pragma unroll
-            for (int p = 0; p < kSlab; ++p) most = nan_max(most, piece_most<T>(w[p]));
-        }
-        top = wave_max(logit_key(most));
-        __syncthreads();
-        if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = top;
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < THREADS / kWave; ++v) top = max(top, sh.wave_key[v]);
+        for (int k = 0; k < kSlab; ++k) most = nan_max(most, piece_most<T>(p[k]));
     }
+    const uint32_t top = block_max(logit_key(most), sh);
     if (top == kKeyNan || top == kKeyNegInf) return answer(-1, NAN);
     if (greedy) return answer(find_by_index(row, 0, [&](float x, int) -> u64 { return logit_key(x) == top; }, sh), 0.f);
     const Weights w{key_logit(top), inverse};
     if (top_k > 0 || w.m == INFINITY) return finish(draw_by_search(row, w, top_k, top_p, min_p, u, sh));
 
-    for (int s = tid; s < kMaxSlabs; s += THREADS) mass.slab[s] = 0;
-    if (!(top_p < 1.f)) {
-        auto kept = [&](float x, int) -> u64 { return w.of_finite(x) >= min_p ? w.fixed_finite(x) : 0; };
-        __syncthreads();
+    // The sum over a slab of what is kept, chunk by chunk; kept(exponent, weight)
+    // says of what. Pieces below `least` hold nothing of it.
+    auto sum_chunks = [&](float least, auto &&kept) {
         for (int s = 0; s < slabs; ++s) {
-            u64 sum = 0;
-            row.pieces(s, [&](const float (&y)[N], int) {
+            double sum = 0.0;
+            words4 p[kSlab];
+            row.load(s, p);
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum += kept(y[i], 0);
-            });
-            sum = wave_add(sum);
-            if ((tid & (kWave - 1)) == 0) atomicAdd(&mass.slab[s], sum);
+            for (int k = 0; k < kSlab; ++k) {
+                if (piece_most<T>(p[k]) < least) continue;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float y = w.exponent(piece_value<T>(p[k], i)), e = fast_exp2(y);
+                    sum += Weights::whole_f64(kept(y, e, s, k, i, p[k]) ? e : 0.f);
+                }
+            }
+            const u64 upto = wave_scan(static_cast<u64>(sum));
+            if (lane == kWave - 1 && R::chunk(s) < kMaxChunks) chunks[R::chunk(s)] = upto;
         }
         __syncthreads();
-        return finish(draw_from_slabs(row, mass.slab, u, kept, sh));
+    };
+    if (!(top_p < 1.f)) {
+        sum_chunks(w.m - 41.f / inverse, [&](float, float e, int, int, int, const words4 &) { return e >= min_p; });
+        return finish(draw_from_chunks(
+            row, chunks, u,
+            [&](float x, int) -> u64 {
+                const float e = fast_exp2(w.exponent(x));
+                return e >= min_p ? Weights::whole(e) : 0;
+            },
+            sh));
     }
 
     // the row's mass by exponent
-    for (int b = tid; b < kMassBins; b += THREADS) mass.bins[b] = 0;
+    for (int b = tid; b < kMassBins; b += THREADS) sh.mass[b] = 0;
     __syncthreads();
+    const float weightless = w.m - 41.f / inverse;
     for (int s = 0; s < slabs; ++s) {
-        row.pieces(s, [&](const float (&y)[N], int) {
+        words4 p[kSlab];
+        row.load(s, p);
+#pragma unroll
+        for (int k = 0; k < kSlab; ++k) {
+            if (piece_most<T>(p[k]) < weightless) continue;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const u64 f = w.fixed_finite(y[i]);
-                if (f) atomicAdd(&mass.bins[mass_bin(y[i], w)], f);
+                const float y = w.exponent(piece_value<T>(p[k], i));
+                const u64 f = Weights::whole(fast_exp2(y));
+                if (f) atomicAdd(&sh.mass[static_cast<int>(mass_bin(y))], f);
             }
-        });
+        }
     }
     __syncthreads();
     constexpr int kOwnBins = kMassBins / THREADS;
     u64 own = 0, total;
 #pragma unroll
-    for (int j = 0; j < kOwnBins; ++j) own += mass.bins[tid * kOwnBins + j];
+    for (int j = 0; j < kOwnBins; ++j) own += sh.mass[tid * kOwnBins + j];
     u64 before = block_scan(own, total, sh);
     const u64 limit = limit_of(top_p, total);
 
     // the prefix ends in one of the bins: what is in the bins before is kept,
     // the bin's own logits are sorted
     for (int j = 0; j < kOwnBins; ++j) {
-        const u64 in_bin = mass.bins[tid * kOwnBins + j];
+        const u64 in_bin = sh.mass[tid * kOwnBins + j];
         if (before < limit && limit <= before + in_bin) {
             sh.pick[0] = static_cast<u64>(tid * kOwnBins + j);
             sh.pick[1] = before;
@@ -944,51 +992,31 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
     }
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    const int cut_bin = static_cast<int>(sh.pick[0]);
+    const float cut_bin = static_cast<float>(static_cast<int>(sh.pick[0]));
     const u64 above = sh.pick[1];
     // below this no logit is in the bins kept (a margin of two bins)
-    const float least = w.m - (static_cast<float>(cut_bin) + 3.f) * (40.f / kMassBins) / w.inverse;
-    for (int s = 0; s < slabs; ++s) {
-        u64 sum = 0;
-        words4 p[kSlab];
-        row.load(s, p);
-#pragma unroll
-        for (int k = 0; k < kSlab; ++k) {
-            if (piece_most<T>(p[k]) < least) continue;
-            const int at = R::at(s, k);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float x = piece_value<T>(p[k], i);
-                const u64 f = w.fixed_finite(x);
-                if (!f) continue;
-                const int b = mass_bin(x, w);
-                if (b < cut_bin) {
-                    if (w.of_finite(x) >= min_p) sum += f;
-                } else if (b == cut_bin) {
-                    const int slot = atomicAdd(&sh.count, 1);
-                    if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(x), at + i);
-                }
-            }
-        }
-        sum = wave_add(sum);
-        if ((tid & (kWave - 1)) == 0) atomicAdd(&mass.slab[s], sum);
-    }
-    __syncthreads();
+    sum_chunks(w.m - (cut_bin + 3.f) * (41.f / kMassBins) / inverse,
+               [&](float y, float e, int s, int k, int i, const words4 &p) {
+                   const float b = mass_bin(y);
+                   if (b >= cut_bin && b < cut_bin + 1.f) {
+                       const int slot = atomicAdd(&sh.count, 1);
+                       if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(piece_value<T>(p, i)), R::at(s, k) + i);
+                   }
+                   return b < cut_bin && e >= min_p;
+               });
     const int n = sh.count;
     if (n > kList<THREADS>) return finish(draw_by_search(row, w, top_k, top_p, min_p, u, sh));
     sort_list(n, sh);
-    const int per = (n + THREADS - 1) / THREADS, from = tid * per;
+    const int per = (n + THREADS - 1) / THREADS, from = tid * per, to = min(n, from + per);
     own = 0;
-    for (int j = 0; j < per; ++j)
-        if (from + j < n) own += w.fixed_finite(key_logit(place_key(sh.list[from + j])));
+    for (int j = from; j < to; ++j) own += w.fixed(key_logit(place_key(sh.list[j])));
     before = above + block_scan(own, total, sh);
-    __syncthreads();
-    for (int j = 0; j < per; ++j) {
-        if (from + j < n && before < limit) {
-            const u64 p = sh.list[from + j];
-            const float x = key_logit(place_key(p));
-            const u64 f = w.fixed_finite(x);
-            if (w.of_finite(x) >= min_p) atomicAdd(&mass.slab[place_index(p, row.n) / R::kSlabLogits], f);
+    for (int j = from; j < to; ++j) {
+        if (before < limit) {
+            const u64 p = sh.list[j];
+            const float e = w.of(key_logit(place_key(p)));
+            const u64 f = Weights::whole(e);
+            if (e >= min_p) atomicAdd(&chunks[min(place_index(p, row.n) / R::kChunk, kMaxChunks - 1)], f);
             before += f;
             if (before >= limit) sh.pick[0] = p;  // the last one kept
         }
@@ -996,22 +1024,24 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
     __syncthreads();
     const u64 cut = sh.pick[0];
     __syncthreads();
-    finish(draw_from_slabs(
-        row, mass.slab, u,
+    finish(draw_from_chunks(
+        row, chunks, u,
         [&](float x, int i) -> u64 {
-            return place(logit_key(x), i) >= cut && w.of_finite(x) >= min_p ? w.fixed_finite(x) : 0;
+            const float e = fast_exp2(w.exponent(x));
+            return place(logit_key(x), i) >= cut && e >= min_p ? Weights::whole(e) : 0;
         },
         sh));
 }
 
-// Threads for a row: its pieces fill a slab or a few, and no row has more
-// than kMaxSlabs slabs; the list holds four times k.
-int threads_for(int vocab, int per_load, int k) {
-    const int pieces = (vocab + per_load - 1) / per_load;
-    const int by_row = pieces <= 64 ? 64 : pieces <= 2048 ? 256 : pieces <= 8192 ? 512 : 1024;
+// Threads for a row: its pieces fill a slab or a few, and the list holds four
+// times k. Many wide rows take fewer, so that several fit a CU and one's
+// reductions hide behind another's stream.
+int threads_for(const LogitRows &x, int per_load, int k) {
+    const int pieces = (x.vocab + per_load - 1) / per_load;
+    const int by_row = pieces <= 64 ? 64 : pieces <= 2048 || x.rows >= 512 ? 256 : pieces <= 8192 ? 512 : 1024;
     return max(by_row, k <= 128 ? 64 : k <= 512 ? 256 : 512);
 }
-static_assert(TROPNN_MAX_VOCAB / (1024 * kSlab * kPerLoad<float>) <= kMaxSlabs, "slabs of the widest row");
+static_assert(TROPNN_MAX_VOCAB / (kWave * kSlab * kPerLoad<float>) <= kMaxChunks, "chunks of the widest row");
 
 template <typename F>
 hipError_t with_threads(int threads, F &&f) {
@@ -1032,7 +1062,7 @@ hipError_t launch_top_logits(const TopArgs &a, void *, hipStream_t stream) {
     const TopKernelArgs k{a.x.p, a.x.stride, a.x.vocab, a.k, a.temperature, a.values, a.indices, a.log_rest};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(min(512, threads_for(a.x.vocab, kPerLoad<T>, a.k)), [&](auto threads) {
+        return with_threads(threads_for(a.x, kPerLoad<T>, a.k), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((top_logits_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
@@ -1048,7 +1078,7 @@ hipError_t launch_sample(const SampleArgs &a, void *, hipStream_t stream) {
                              a.temperature, a.top_p, a.min_p, a.top_k, a.tokens, a.log_probs};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(threads_for(a.x.vocab, kPerLoad<T>, 1), [&](auto threads) {
+        return with_threads(threads_for(a.x, kPerLoad<T>, 1), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((sample_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
