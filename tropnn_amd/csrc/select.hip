@@ -28,6 +28,7 @@ constexpr int kSlab = 8;        // pieces of a thread that are in flight togethe
 constexpr int kKeyBins = 2048;  // of keys, by their distance from the largest
 constexpr int kKeyShift = 15;   // 2^15 keys a bin, 256 bins an octave
 constexpr int kMassBins = 2048; // of a row's weights, by exponent
+constexpr int kSpare = 2048;    // logits that can be among the list's first
 constexpr int kRanked = 1024;   // logits sorted by counting
 constexpr int kMaxChunks = 512; // a wave's share of a slab, in the widest row
 constexpr float kFixed = 1099511627776.f;  // 2^40: sampling weights are multiples of 2^-40
@@ -69,6 +70,7 @@ struct Shared {
         uint32_t key_counts[kKeyBins];
         uint32_t ranks[kRanked];
         u64 mass[kMassBins];
+        u64 spare[kSpare];
     };
     u64 wave[kWaves < 2 ? 2 : kWaves];
     u64 pick[3];
@@ -95,21 +97,36 @@ struct Row {
     static __device__ __forceinline__ int at(int slab, int u) {
         return chunk(slab) * kChunk + (u * kWave + (static_cast<int>(threadIdx.x) & (kWave - 1))) * N;
     }
+    __device__ __forceinline__ bool full(int slab) const { return (slab + 1) * kSlabLogits <= n; }
+    // Piece u of a slab; all -inf where it is not whole.
+    __device__ __forceinline__ words4 load_one(int slab, int u, bool full) const {
+        const int from = at(slab, u);
+        if (full || from + N <= n) return load_piece(x + from);
+        float none[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) none[i] = -INFINITY;
+        return make_piece<T>(none);
+    }
+    // The row's last logits, where they do not fill a piece, in the slab that
+    // has them; the rest of that piece is -inf.
+    __device__ __forceinline__ void load_end(int slab, words4 (&w)[kSlab]) const {
+        const int from = n - n % N;
+        if (from == n || full(slab)) return;
+        bool mine = false;
+#pragma unroll
+        for (int u = 0; u < kSlab; ++u) mine |= at(slab, u) == from;
+        if (!mine) return;
+        const words4 end = load_piece_to(x, from, n);
+#pragma unroll
+        for (int u = 0; u < kSlab; ++u)
+            if (at(slab, u) == from) w[u] = end;
+    }
     // Logits past the row's end are -inf.
     __device__ __forceinline__ void load(int slab, words4 (&w)[kSlab]) const {
-        if ((slab + 1) * kSlabLogits <= n) {
+        const bool whole = full(slab);
 #pragma unroll
-            for (int u = 0; u < kSlab; ++u) w[u] = load_piece(x + at(slab, u));
-        } else {
-            float none[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) none[i] = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < kSlab; ++u) {
-                w[u] = make_piece<T>(none);
-                if (at(slab, u) < n) w[u] = load_piece_to(x, at(slab, u), n);
-            }
-        }
+        for (int u = 0; u < kSlab; ++u) w[u] = load_one(slab, u, whole);
+        load_end(slab, w);
     }
     // f(value, index) for every logit
     template <typename F>
@@ -193,7 +210,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, Shared<THREADS> &sh) {
 // The first index, in order, at which the running sum of mass(value, index)
 // passes `target` (which is below the row's sum).
 template <typename T, int THREADS, typename M>
-__device__ int find_by_index(const Row<T, THREADS> &row, u64 target, M &&mass, Shared<THREADS> &sh) {
+__device__ __forceinline__ int find_by_index(const Row<T, THREADS> &row, u64 target, M &&mass, Shared<THREADS> &sh) {
     constexpr int N = Row<T, THREADS>::N;
     u64 running = 0;
     __syncthreads();
@@ -230,7 +247,7 @@ __device__ int find_by_index(const Row<T, THREADS> &row, u64 target, M &&mass, S
 // reaches `limit` (1 <= limit <= the row's mass). mass(value, index) of equal
 // values is equal, or 0.
 template <typename T, int THREADS, typename M>
-__device__ u64 find_cut(const Row<T, THREADS> &row, u64 limit, M &&mass, Shared<THREADS> &sh) {
+__device__ __forceinline__ u64 find_cut(const Row<T, THREADS> &row, u64 limit, M &&mass, Shared<THREADS> &sh) {
     const int tid = threadIdx.x;
     uint32_t key = 0;
     u64 above = 0, ties = 0;  // mass before the digits found so far; of those that share them all
@@ -276,7 +293,7 @@ __device__ u64 find_cut(const Row<T, THREADS> &row, u64 limit, M &&mass, Shared<
 // at a distance of up to 64 lie in 128 numbers that no other wave touches, so
 // only the longer distances need the workgroup's barrier.
 template <int THREADS>
-__device__ void sort_down(u64 *v, int n) {
+__device__ __forceinline__ void sort_down(u64 *v, int n) {
     bool far = true;
     for (int size = 2; size <= n; size <<= 1) {
         for (int d = size >> 1; d > 0; d >>= 1) {
@@ -307,7 +324,7 @@ __device__ __forceinline__ int slots_for(int n) { return n <= 1 ? 1 : 1 << (32 -
 // chain of LDS round trips (80 numbers, 512 threads: 5 us with the network)
 // until they are many.
 template <int THREADS>
-__device__ void sort_list(int n, Shared<THREADS> &sh) {
+__device__ __forceinline__ void sort_list(int n, Shared<THREADS> &sh) {
     const int tid = threadIdx.x, slots = slots_for(max(n, kWave));
     __syncthreads();
     if (n > kRanked || slots > THREADS) {
@@ -337,7 +354,7 @@ __device__ void sort_list(int n, Shared<THREADS> &sh) {
 // of one exponent over many bins (the threads' additions to one bin go one by
 // one). Where the k-th is farther, digit by digit: 16 bits of it.
 template <int THREADS, typename K>
-__device__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
+__device__ __forceinline__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
     constexpr int kOwn = kKeyBins / THREADS;
     const int tid = threadIdx.x;
     const uint32_t wanted = static_cast<uint32_t>(k);
@@ -402,20 +419,18 @@ __device__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
     return bound;
 }
 
-// The sum of all threads' parts (not negative), the same bits however they are
-// dealt to the threads: as integers in units of 2^-40 of the largest. NaN where
-// one is NaN or infinite.
-template <int COUNT, int THREADS>
-__device__ float sum_in_any_order(const float (&parts)[COUNT], Shared<THREADS> &sh) {
+// The sum of n parts (not negative; part(j), the same whenever it is asked
+// for), the same bits in whatever order they lie: as integers in units of
+// 2^-40 of the largest. NaN where one is NaN or infinite.
+template <int THREADS, typename P>
+__device__ __forceinline__ float sum_in_any_order(int n, P &&part, Shared<THREADS> &sh) {
     uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) most = max(most, __builtin_bit_cast(uint32_t, parts[j]) & 0x7fffffffu);
+    for (int j = threadIdx.x; j < n; j += THREADS) most = max(most, __builtin_bit_cast(uint32_t, part(j)) & 0x7fffffffu);
     most = block_max(most, sh);
     if (most >= 0x7f800000u) return NAN;
     const int up = 40 - (static_cast<int>(most >> 23) - 127);
     u64 q = 0;
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) q += static_cast<u64>(ldexp(static_cast<double>(parts[j]), up));
+    for (int j = threadIdx.x; j < n; j += THREADS) q += static_cast<u64>(ldexp(static_cast<double>(part(j)), up));
     return static_cast<float>(ldexp(static_cast<double>(block_sum(q, sh)), -up));
 }
 
@@ -434,12 +449,12 @@ __device__ float sum_in_any_order(const float (&parts)[COUNT], Shared<THREADS> &
 // changes from run to run. Returns the number collected, in no
 // particular order, or -1 if they were too many.
 template <bool MOST, bool SUM, typename T, int THREADS, typename Begin, typename Sum>
-__device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, float &bound, float &total, float &extra,
+__device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, float &bound, float &total, float &extra,
                        Begin &&begin, Sum &&sum) {
     using R = Row<T, THREADS>;
-    constexpr int N = R::N, kOwn = kList<THREADS> / THREADS;
+    constexpr int N = R::N;
     const int slabs = row.slabs(), n = row.n, tid = threadIdx.x;
-    words4 w[kSlab], next[kSlab];
+    words4 w[kSlab];
     row.load(0, w);
     if (tid == 0) sh.count = 0;
     uint32_t most_key = 0;
@@ -465,25 +480,19 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
     bound = begin(bound, key_logit(most_key));
     total = extra = 0.f;
 
-    // the pieces put aside, this thread's share of them, are summed or read
-    // again: those that reach the bound into the list
-    u64 own[kOwn];
-    int aside = 0;
-    auto take_own = [&] {
-#pragma unroll
-        for (int j = 0; j < kOwn; ++j) own[j] = j * THREADS + tid < aside ? sh.list[j * THREADS + tid] : 0;
-    };
-    auto raise = [&] {
+    auto raise = [&](int aside) {
         const float next = key_logit(bound_of<THREADS>(
             k,
             [&](auto &&f) {
-#pragma unroll
-                for (int j = 0; j < kOwn; ++j)
-                    if (own[j]) f(place_key(own[j]));
+                for (int j = tid; j < aside; j += THREADS) f(place_key(sh.list[j]));
             },
             sh));
         if (!(next < bound)) bound = next;
+        __syncthreads();
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
     };
+    // the values of a piece put aside
     auto read_again = [&](u64 entry, float (&y)[N]) {
         const int at = static_cast<int>(static_cast<uint32_t>(entry)) * N;
         const words4 p = load_piece_to(row.x, at, n);
@@ -491,10 +500,29 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
         for (int i = 0; i < N; ++i) y[i] = piece_value<T>(p, i);
         return at;
     };
+    // what is left in the list after the pieces put aside: their parts of the sum
+    auto add_parts = [&](int aside) {
+        __syncthreads();
+        if constexpr (SUM)
+            extra += sum_in_any_order(
+                aside,
+                [&](int j) {
+                    const uint32_t bits = static_cast<uint32_t>(sh.list[j]);
+                    return __builtin_bit_cast(float, bits);
+                },
+                sh);
+    };
+    // the spare list becomes the list
+    auto take_spare = [&](int count) {
+        __syncthreads();
+        for (int j = tid; j < count; j += THREADS) sh.list[j] = sh.spare[j];
+        __syncthreads();
+    };
 
     __syncthreads();
     for (int slab = 0; slab < slabs; ++slab) {
-        if (slab + 1 < slabs) row.load(slab + 1, next);
+        // each piece's registers take the next slab's as soon as it is done
+        const bool more = slab + 1 < slabs, whole = row.full(slab + 1);
 #pragma unroll
         for (int u = 0; u < kSlab; ++u) {
             const float most = piece_most<T>(w[u]);
@@ -510,66 +538,70 @@ __device__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, f
                 for (int i = 0; i < N; ++i) y[i] = piece_value<T>(w[u], i);
                 const float part = sum(y);
                 total += reaches ? 0.f : part;
+                // here and now: left to itself, the compiler moves the sums after
+                // the last piece, with all the slab's values in registers
+                asm volatile("" : "+v"(total));
             }
+            if (more) w[u] = row.load_one(slab + 1, u, whole);
         }
-        if (slab + 1 < slabs) {
+        if (more) {
+            row.load_end(slab + 1, w);
             __syncthreads();
-            aside = sh.count;
+            const int aside = sh.count;
             if (aside > kList<THREADS>) return -1;
             __syncthreads();
             if (aside > kList<THREADS> / 2) {
-                take_own();
-                raise();
-                if (tid == 0) sh.count = 0;
-                __syncthreads();
-                float parts[kOwn];
-#pragma unroll
-                for (int j = 0; j < kOwn; ++j) {
-                    parts[j] = 0.f;
-                    if (!own[j]) continue;
-                    if (!(key_logit(place_key(own[j])) < bound)) {
-                        sh.list[atomicAdd(&sh.count, 1)] = own[j];
+                raise(aside);
+                for (int j = tid; j < aside; j += THREADS) {
+                    const u64 entry = sh.list[j];
+                    float part = 0.f;
+                    if (!(key_logit(place_key(entry)) < bound)) {
+                        const int slot = atomicAdd(&sh.count, 1);
+                        if (slot < kSpare) sh.spare[slot] = entry;
                     } else if constexpr (SUM) {
                         float y[N];
-                        read_again(own[j], y);
-                        parts[j] = sum(y);
+                        read_again(entry, y);
+                        part = sum(y);
                     }
+                    sh.list[j] = __builtin_bit_cast(uint32_t, part);
                 }
-                if constexpr (SUM) extra += sum_in_any_order(parts, sh);
                 __syncthreads();
+                const int kept = sh.count;
+                if (kept > kSpare) return -1;
+                // the sum's scratch is not the spare list's
+                add_parts(aside);
+                take_spare(kept);
             }
-#pragma unroll
-            for (int u = 0; u < kSlab; ++u) w[u] = next[u];
         }
     }
     __syncthreads();
-    aside = sh.count;
+    const int aside = sh.count;
     if (aside > kList<THREADS>) return -1;
-    take_own();
-    if (!few && aside > k) raise();
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    float parts[kOwn];
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-        parts[j] = 0.f;
-        if (!own[j]) continue;
+    if (!few && aside > k) {
+        raise(aside);
+    } else {
+        __syncthreads();
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+    }
+    for (int j = tid; j < aside; j += THREADS) {
         float y[N];
-        const int at = read_again(own[j], y);
+        const int at = read_again(sh.list[j], y);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (!(y[i] < bound) && at + i < n) {
                 const int slot = atomicAdd(&sh.count, 1);
-                if (slot < kList<THREADS>) sh.list[slot] = place(logit_key(y[i]), at + i);
+                if (slot < kSpare) sh.spare[slot] = place(logit_key(y[i]), at + i);
                 y[i] = -INFINITY;
             }
         }
-        if constexpr (SUM) parts[j] = sum(y);
+        if constexpr (SUM) sh.list[j] = __builtin_bit_cast(uint32_t, sum(y));
     }
-    if constexpr (SUM) extra += sum_in_any_order(parts, sh);
-    __syncthreads();
-    return sh.count <= kList<THREADS> ? sh.count : -1;
+    add_parts(aside);
+    const int count = sh.count;
+    if (count > kSpare) return -1;
+    take_spare(count);
+    return count;
 }
 
 struct TopKernelArgs {
@@ -717,7 +749,7 @@ struct Drawn {
 
 // The exact search for any row and parameters.
 template <typename T, int THREADS>
-__device__ Drawn draw_by_search(const Row<T, THREADS> &row, const Weights &w, int top_k, float top_p, float min_p, float u,
+__device__ __forceinline__ Drawn draw_by_search(const Row<T, THREADS> &row, const Weights &w, int top_k, float top_p, float min_p, float u,
                                 Shared<THREADS> &sh) {
     u64 cut = 0;
     if (top_k > 0 && top_k < row.n)
@@ -741,7 +773,7 @@ __device__ Drawn draw_by_search(const Row<T, THREADS> &row, const Weights &w, in
 // Draws among the first n of the sorted list, which are all that top_k leaves
 // (but for logits without weight). The first wave has the list's sums.
 template <int THREADS>
-__device__ Drawn draw_from_list(int n, const Weights &w, float top_p, float min_p, float u, int vocab, Shared<THREADS> &sh) {
+__device__ __forceinline__ Drawn draw_from_list(int n, const Weights &w, float top_p, float min_p, float u, int vocab, Shared<THREADS> &sh) {
     const int tid = threadIdx.x;
     if (tid < kWave) {
         const int per = (n + kWave - 1) / kWave, from = tid * per, to = min(n, from + per);
@@ -811,7 +843,7 @@ __device__ __forceinline__ float mass_bin(float y) { return y * (-kMassBins / 41
 // Draws from all logits of which mass(value, index) is not 0, given its sum
 // over every chunk.
 template <typename T, int THREADS, typename M>
-__device__ Drawn draw_from_chunks(const Row<T, THREADS> &row, const u64 *chunks, float u, M &&mass, Shared<THREADS> &sh) {
+__device__ __forceinline__ Drawn draw_from_chunks(const Row<T, THREADS> &row, const u64 *chunks, float u, M &&mass, Shared<THREADS> &sh) {
     using R = Row<T, THREADS>;
     constexpr int kEach = R::kChunk / THREADS;
     const int tid = threadIdx.x;
