@@ -203,6 +203,40 @@ __device__ __forceinline__ ExpSum wave_join(ExpSum v, float c) {
     return v;
 }
 
+// Lane l gets lane l - n's value within its row of 16 (CTRL row_shr:n), or the
+// last of the row or the two rows before it (row_bcast, to the ROWS given), else
+// `none`. Six of them fold a wave into its last lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t v, uint32_t none = 0) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_from(float v, float none) {
+    return __builtin_bit_cast(float, dpp_from<CTRL, ROWS>(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, none)));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_from(unsigned long long v) {
+    const uint32_t low = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v)), high = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v >> 32));
+    return static_cast<unsigned long long>(high) << 32 | low;
+}
+template <typename F>
+__device__ __forceinline__ float wave_fold(float v, float none, F &&f) {
+    v = f(v, dpp_from<0x111, 0xF>(v, none));
+    v = f(v, dpp_from<0x112, 0xF>(v, none));
+    v = f(v, dpp_from<0x114, 0xF>(v, none));
+    v = f(v, dpp_from<0x118, 0xF>(v, none));
+    v = f(v, dpp_from<0x142, 0xA>(v, none));
+    v = f(v, dpp_from<0x143, 0xC>(v, none));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), kWave - 1));
+}
+// The wave's sum and largest value (NaN left out), in scalar registers.
+__device__ __forceinline__ float wave_total(float v) {
+    return wave_fold(v, 0.f, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_most_of(float v) {
+    return wave_fold(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+
 __device__ __forceinline__ float wave_sum(float v) { return group_sum(v, kWave); }
 
 template <typename V>

@@ -28,7 +28,6 @@ constexpr int kSlab = 8;        // pieces of a thread that are in flight togethe
 constexpr int kKeyBins = 2048;  // of keys, by their distance from the largest
 constexpr int kKeyShift = 15;   // 2^15 keys a bin, 256 bins an octave
 constexpr int kMassBins = 2048; // of a row's weights, by exponent
-constexpr int kSpare = 2048;    // logits that can be among the list's first
 constexpr int kRanked = 1024;   // logits sorted by counting
 constexpr int kMaxChunks = 512; // a wave's share of a slab, in the widest row
 constexpr float kFixed = 1099511627776.f;  // 2^40: sampling weights are multiples of 2^-40
@@ -47,9 +46,13 @@ __device__ __forceinline__ int place_index(u64 p, int n) {
 // NaN if either is.
 __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Logits that a workgroup can collect: eight a thread.
+// Logits that a workgroup can collect: four a thread, so that of the workgroups
+// of 256 as many fit a CU's LDS as its registers hold.
 template <int THREADS>
-constexpr int kList = THREADS < 512 ? 8 * THREADS : 4096;
+constexpr int kList = 4 * THREADS;
+// Of these, logits that can be among the first.
+template <int THREADS>
+constexpr int kSpare = kList<THREADS> < 2048 ? kList<THREADS> : 2048;
 
 // The largest logit of a piece, NaN if one is.
 template <typename T>
@@ -60,8 +63,9 @@ __device__ __forceinline__ float piece_most(const words4 &w) {
     return most;
 }
 
-template <int THREADS>
+template <int THREADS, bool MASS>
 struct Shared {
+    static constexpr int kThreads = THREADS;
     static constexpr int kWaves = THREADS / kWave;
     u64 list[kList<THREADS>];
     union {
@@ -69,8 +73,8 @@ struct Shared {
         uint32_t counts[kBins];
         uint32_t key_counts[kKeyBins];
         uint32_t ranks[kRanked];
-        u64 mass[kMassBins];
-        u64 spare[kSpare];
+        u64 mass[MASS ? kMassBins : 1];
+        u64 spare[kSpare<THREADS>];
     };
     u64 wave[kWaves < 2 ? 2 : kWaves];
     u64 pick[3];
@@ -140,18 +144,6 @@ struct Row {
     }
 };
 
-// Lane l gets lane l - n's value within its row of 16 (CTRL row_shr:n), or the
-// last of the row or the two rows before it (row_bcast), else 0.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_from(uint32_t v) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 dpp_from(u64 v) {
-    const uint32_t low = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v)), high = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v >> 32));
-    return static_cast<u64>(high) << 32 | low;
-}
-
 // The lanes' sum up to and with this one.
 template <typename V>
 __device__ __forceinline__ V wave_scan(V v) {
@@ -169,8 +161,9 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
 }
 
 // The sum of the threads' values before this one's, and of all.
-template <int THREADS>
-__device__ __forceinline__ u64 block_scan(u64 v, u64 &total, Shared<THREADS> &sh) {
+template <typename SH>
+__device__ __forceinline__ u64 block_scan(u64 v, u64 &total, SH &sh) {
+    constexpr int THREADS = SH::kThreads;
     constexpr int kWaves = THREADS / kWave;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const u64 up = wave_scan(v);
@@ -187,15 +180,16 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 &total, Shared<THREADS> &sh
     return before + up - v;
 }
 
-template <int THREADS>
-__device__ __forceinline__ u64 block_sum(u64 v, Shared<THREADS> &sh) {
+template <typename SH>
+__device__ __forceinline__ u64 block_sum(u64 v, SH &sh) {
     u64 total;
     block_scan(v, total, sh);
     return total;
 }
 
-template <int THREADS>
-__device__ __forceinline__ uint32_t block_max(uint32_t v, Shared<THREADS> &sh) {
+template <typename SH>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, SH &sh) {
+    constexpr int THREADS = SH::kThreads;
     v = wave_max(v);
     __syncthreads();
     if ((threadIdx.x & (kWave - 1)) == 0) sh.wave_key[threadIdx.x / kWave] = v;
@@ -209,8 +203,8 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, Shared<THREADS> &sh) {
 
 // The first index, in order, at which the running sum of mass(value, index)
 // passes `target` (which is below the row's sum).
-template <typename T, int THREADS, typename M>
-__device__ __forceinline__ int find_by_index(const Row<T, THREADS> &row, u64 target, M &&mass, Shared<THREADS> &sh) {
+template <typename T, int THREADS, typename M, typename SH>
+__device__ __forceinline__ int find_by_index(const Row<T, THREADS> &row, u64 target, M &&mass, SH &sh) {
     constexpr int N = Row<T, THREADS>::N;
     u64 running = 0;
     __syncthreads();
@@ -246,8 +240,8 @@ __device__ __forceinline__ int find_by_index(const Row<T, THREADS> &row, u64 tar
 // The place of the last logit of the shortest prefix of the order whose mass
 // reaches `limit` (1 <= limit <= the row's mass). mass(value, index) of equal
 // values is equal, or 0.
-template <typename T, int THREADS, typename M>
-__device__ __forceinline__ u64 find_cut(const Row<T, THREADS> &row, u64 limit, M &&mass, Shared<THREADS> &sh) {
+template <typename T, int THREADS, typename M, typename SH>
+__device__ __forceinline__ u64 find_cut(const Row<T, THREADS> &row, u64 limit, M &&mass, SH &sh) {
     const int tid = threadIdx.x;
     uint32_t key = 0;
     u64 above = 0, ties = 0;  // mass before the digits found so far; of those that share them all
@@ -323,8 +317,9 @@ __device__ __forceinline__ int slots_for(int n) { return n <= 1 ? 1 : 1 << (32 -
 // n^2 / THREADS comparisons against broadcast reads beat the sorting network's
 // chain of LDS round trips (80 numbers, 512 threads: 5 us with the network)
 // until they are many.
-template <int THREADS>
-__device__ __forceinline__ void sort_list(int n, Shared<THREADS> &sh) {
+template <typename SH>
+__device__ __forceinline__ void sort_list(int n, SH &sh) {
+    constexpr int THREADS = SH::kThreads;
     const int tid = threadIdx.x, slots = slots_for(max(n, kWave));
     __syncthreads();
     if (n > kRanked || slots > THREADS) {
@@ -353,8 +348,9 @@ __device__ __forceinline__ void sort_list(int n, Shared<THREADS> &sh) {
 // resolve 2^-8 of it over eight octaves, as finely as bf16, and spread even keys
 // of one exponent over many bins (the threads' additions to one bin go one by
 // one). Where the k-th is farther, digit by digit: 16 bits of it.
-template <int THREADS, typename K>
-__device__ __forceinline__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &sh) {
+template <typename K, typename SH>
+__device__ __forceinline__ uint32_t bound_of(int k, K &&keys, SH &sh) {
+    constexpr int THREADS = SH::kThreads;
     constexpr int kOwn = kKeyBins / THREADS;
     const int tid = threadIdx.x;
     const uint32_t wanted = static_cast<uint32_t>(k);
@@ -422,8 +418,9 @@ __device__ __forceinline__ uint32_t bound_of(int k, K &&keys, Shared<THREADS> &s
 // The sum of n parts (not negative; part(j), the same whenever it is asked
 // for), the same bits in whatever order they lie: as integers in units of
 // 2^-40 of the largest. NaN where one is NaN or infinite.
-template <int THREADS, typename P>
-__device__ __forceinline__ float sum_in_any_order(int n, P &&part, Shared<THREADS> &sh) {
+template <typename P, typename SH>
+__device__ __forceinline__ float sum_in_any_order(int n, P &&part, SH &sh) {
+    constexpr int THREADS = SH::kThreads;
     uint32_t most = 0;
     for (int j = threadIdx.x; j < n; j += THREADS) most = max(most, __builtin_bit_cast(uint32_t, part(j)) & 0x7fffffffu);
     most = block_max(most, sh);
@@ -448,8 +445,8 @@ __device__ __forceinline__ float sum_in_any_order(int n, P &&part, Shared<THREAD
 // stream, extra that of the pieces put aside, whose order among the threads
 // changes from run to run. Returns the number collected, in no
 // particular order, or -1 if they were too many.
-template <bool MOST, bool SUM, typename T, int THREADS, typename Begin, typename Sum>
-__device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared<THREADS> &sh, float &bound, float &total, float &extra,
+template <bool MOST, bool SUM, typename T, int THREADS, typename Begin, typename Sum, typename SH>
+__device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, SH &sh, float &bound, float &total, float &extra,
                        Begin &&begin, Sum &&sum) {
     using R = Row<T, THREADS>;
     constexpr int N = R::N;
@@ -465,7 +462,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared
         most_key = block_max(most_key, sh);
     }
     const bool few = (min(n, R::kSlabLogits) + N - 1) / N < k;  // pieces: then the row is one slab, bounded logit by logit
-    bound = key_logit(bound_of<THREADS>(
+    bound = key_logit(bound_of(
         min(k, n),
         [&](auto &&f) {
             if (few) {
@@ -481,7 +478,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared
     total = extra = 0.f;
 
     auto raise = [&](int aside) {
-        const float next = key_logit(bound_of<THREADS>(
+        const float next = key_logit(bound_of(
             k,
             [&](auto &&f) {
                 for (int j = tid; j < aside; j += THREADS) f(place_key(sh.list[j]));
@@ -557,7 +554,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared
                     float part = 0.f;
                     if (!(key_logit(place_key(entry)) < bound)) {
                         const int slot = atomicAdd(&sh.count, 1);
-                        if (slot < kSpare) sh.spare[slot] = entry;
+                        if (slot < kSpare<THREADS>) sh.spare[slot] = entry;
                     } else if constexpr (SUM) {
                         float y[N];
                         read_again(entry, y);
@@ -567,7 +564,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared
                 }
                 __syncthreads();
                 const int kept = sh.count;
-                if (kept > kSpare) return -1;
+                if (kept > kSpare<THREADS>) return -1;
                 // the sum's scratch is not the spare list's
                 add_parts(aside);
                 take_spare(kept);
@@ -591,7 +588,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared
         for (int i = 0; i < N; ++i) {
             if (!(y[i] < bound) && at + i < n) {
                 const int slot = atomicAdd(&sh.count, 1);
-                if (slot < kSpare) sh.spare[slot] = place(logit_key(y[i]), at + i);
+                if (slot < kSpare<THREADS>) sh.spare[slot] = place(logit_key(y[i]), at + i);
                 y[i] = -INFINITY;
             }
         }
@@ -599,7 +596,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, Shared
     }
     add_parts(aside);
     const int count = sh.count;
-    if (count > kSpare) return -1;
+    if (count > kSpare<THREADS>) return -1;
     take_spare(count);
     return count;
 }
@@ -617,7 +614,7 @@ struct TopKernelArgs {
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a) {
     constexpr int N = Row<T, THREADS>::N;
-    __shared__ Shared<THREADS> sh;
+    __shared__ Shared<THREADS, false> sh;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const Row<T, THREADS> row{static_cast<const T *>(a.x) + r * a.stride, a.vocab};
@@ -748,9 +745,9 @@ struct Drawn {
 };
 
 // The exact search for any row and parameters.
-template <typename T, int THREADS>
+template <typename T, int THREADS, typename SH>
 __device__ __forceinline__ Drawn draw_by_search(const Row<T, THREADS> &row, const Weights &w, int top_k, float top_p, float min_p, float u,
-                                Shared<THREADS> &sh) {
+                                SH &sh) {
     u64 cut = 0;
     if (top_k > 0 && top_k < row.n)
         cut = find_cut(row, static_cast<u64>(top_k), [](float, int) -> u64 { return 1; }, sh);
@@ -772,8 +769,9 @@ __device__ __forceinline__ Drawn draw_by_search(const Row<T, THREADS> &row, cons
 
 // Draws among the first n of the sorted list, which are all that top_k leaves
 // (but for logits without weight). The first wave has the list's sums.
-template <int THREADS>
-__device__ __forceinline__ Drawn draw_from_list(int n, const Weights &w, float top_p, float min_p, float u, int vocab, Shared<THREADS> &sh) {
+template <typename SH>
+__device__ __forceinline__ Drawn draw_from_list(int n, const Weights &w, float top_p, float min_p, float u, int vocab, SH &sh) {
+    constexpr int THREADS = SH::kThreads;
     const int tid = threadIdx.x;
     if (tid < kWave) {
         const int per = (n + kWave - 1) / kWave, from = tid * per, to = min(n, from + per);
@@ -842,8 +840,8 @@ __device__ __forceinline__ float mass_bin(float y) { return y * (-kMassBins / 41
 
 // Draws from all logits of which mass(value, index) is not 0, given its sum
 // over every chunk.
-template <typename T, int THREADS, typename M>
-__device__ __forceinline__ Drawn draw_from_chunks(const Row<T, THREADS> &row, const u64 *chunks, float u, M &&mass, Shared<THREADS> &sh) {
+template <typename T, int THREADS, typename M, typename SH>
+__device__ __forceinline__ Drawn draw_from_chunks(const Row<T, THREADS> &row, const u64 *chunks, float u, M &&mass, SH &sh) {
     using R = Row<T, THREADS>;
     constexpr int kEach = R::kChunk / THREADS;
     const int tid = threadIdx.x;
@@ -892,7 +890,7 @@ template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) {
     using R = Row<T, THREADS>;
     constexpr int N = R::N;
-    __shared__ Shared<THREADS> sh;
+    __shared__ Shared<THREADS, true> sh;
     __shared__ u64 chunks[kMaxChunks];
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const int64_t r = blockIdx.x;
@@ -1071,7 +1069,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
 int threads_for(const LogitRows &x, int per_load, int k) {
     const int pieces = (x.vocab + per_load - 1) / per_load;
     const int by_row = pieces <= 64 ? 64 : pieces <= 2048 || x.rows >= 512 ? 256 : pieces <= 8192 ? 512 : 1024;
-    return max(by_row, k <= 128 ? 64 : k <= 512 ? 256 : 512);
+    return max(by_row, k <= 64 ? 64 : k <= 256 ? 256 : k <= 512 ? 512 : 1024);
 }
 static_assert(TROPNN_MAX_VOCAB / (kWave * kSlab * kPerLoad<float>) <= kMaxChunks, "chunks of the widest row");
 
@@ -1110,7 +1108,7 @@ hipError_t launch_sample(const SampleArgs &a, void *, hipStream_t stream) {
                              a.temperature, a.top_p, a.min_p, a.top_k, a.tokens, a.log_probs};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(threads_for(a.x, kPerLoad<T>, 1), [&](auto threads) {
+        return with_threads(threads_for(a.x, kPerLoad<T>, a.top_ks ? 1 : max(a.top_k, 1)), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((sample_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
