@@ -8,11 +8,12 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from typing import Any
 
 import torch
 from torch import Tensor
 
-from .pairwise_hip import _LOCK, _check, _ptr, _stream, library_path, load_library
+from .pairwise_hip import _LOCK, _check, _pairwise_op, _ptr, _stream, library_path, load_library
 
 LOGITS_ABI_VERSION = 1
 LOGITS_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -29,6 +30,7 @@ LOGITS_SYMBOLS = (
     "tropnn_hip_sample",
 )
 _LIB: ctypes.CDLL | None = None
+_DISTILL_OP: Any = None
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -69,6 +71,24 @@ def load_logits_library() -> ctypes.CDLL:
             )
         _LIB = lib
     return _LIB
+
+
+def distill_op() -> Any:
+    """torch.ops.tropnn_hip.distill (csrc/logits_op.cpp), loaded once and bound
+    to the entry points of the library that load_logits_library() checked."""
+    global _DISTILL_OP
+    if _DISTILL_OP is not None:
+        return _DISTILL_OP
+    lib = load_logits_library()
+    _pairwise_op()  # loads the operator library
+    with _LOCK:
+        if _DISTILL_OP is None:
+            names = ("tropnn_hip_distill", "tropnn_hip_distill_workspace_size", "tropnn_hip_scale_in_place",
+                     "tropnn_hip_last_error")
+            torch.ops.tropnn_hip.bind_logits_abi(
+                *(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), LOGITS_ABI_VERSION)
+            _DISTILL_OP = torch.ops.tropnn_hip.distill.default
+    return _DISTILL_OP
 
 
 def on_device_of(fn):
@@ -121,28 +141,6 @@ def top_logits_hip(logits: Tensor, k: int, temperature: float) -> tuple[Tensor, 
                                    indices.data_ptr(), log_rest.data_ptr(), _ptr(ws), size, _stream(device))
     _check(rc, "tropnn_hip_top_logits")
     return values, indices, log_rest
-
-
-@on_device_of
-def distill_hip(logits: Tensor, values: Tensor, indices: Tensor, log_rest: Tensor | None, weights: Tensor | None,
-                temperature: float, scale: float, mean: bool, want_grad: bool) -> tuple[Tensor, Tensor | None]:
-    """(loss, its gradient with respect to the logits or None)."""
-    lib, device = load_logits_library(), logits.device
-    x, rows, vocab, stride = as_rows(logits)
-    dtype, k = LOGITS_DTYPES[x.dtype], values.shape[-1]
-    values, indices = values.contiguous(), indices.contiguous()
-    log_rest = None if log_rest is None else log_rest.contiguous()
-    weights = None if weights is None else weights.contiguous()
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    grad = torch.empty(logits.shape, dtype=x.dtype, device=device) if want_grad else None
-    size = lib.tropnn_hip_distill_workspace_size(rows, vocab, dtype, k, int(want_grad))
-    ws = _workspace(size, device)
-    rc = lib.tropnn_hip_distill(rows, vocab, stride, x.data_ptr(), dtype, k, values.data_ptr(),
-                                LOGITS_DTYPES[values.dtype], indices.data_ptr(), _ptr(log_rest), _ptr(weights),
-                                temperature, scale, int(mean), loss.data_ptr(), _ptr(grad), _ptr(ws), size,
-                                _stream(device))
-    _check(rc, "tropnn_hip_distill")
-    return loss, grad
 
 
 @on_device_of

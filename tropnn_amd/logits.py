@@ -29,12 +29,11 @@ from .backends.logits_hip import (
     LOGITS_DTYPES,
     MAX_TOP,
     MAX_VOCAB,
-    distill_hip,
+    distill_op,
     sample_hip,
-    scale_in_place,
     top_logits_hip,
 )
-from .losses import _is_unit
+from .losses import _UNITS
 
 
 class TopLogits(NamedTuple):
@@ -90,34 +89,6 @@ def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> TopLogits
     return TopLogits(*top_logits_hip(logits.detach(), k, _check_temperature("top_logits", temperature)))
 
 
-class _Distillation(torch.autograd.Function):
-    """The forward's launch writes the gradient too, and backward hands it
-    over: it is scaled in place by the incoming gradient (which the kernel
-    reads, and leaves the gradient alone where it is one), and given up, so that
-    autograd can keep it as the logits' grad without a copy. A second backward
-    through the same graph computes it again from the saved inputs."""
-
-    @staticmethod
-    def forward(ctx, logits, values, indices, log_rest, weights, temperature, scale, mean):
-        want_grad = ctx.needs_input_grad[0]
-        loss, grad = distill_hip(logits.detach(), values, indices, log_rest, weights, temperature, scale, mean, want_grad)
-        if want_grad:
-            ctx.grad = grad
-            ctx.how = (temperature, scale, mean)
-            ctx.save_for_backward(logits, values, indices, log_rest, weights)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            _, grad = distill_hip(*ctx.saved_tensors, *ctx.how, True)
-        if not _is_unit(grad_out):
-            scale_in_place(grad, grad_out.contiguous())
-        return grad, None, None, None, None, None, None, None
-
-
 def distillation_loss(
     logits: Tensor,
     values: Tensor,
@@ -169,8 +140,8 @@ def distillation_loss(
         weights = weights.detach()
     if reduction not in ("mean", "sum"):
         raise ValueError(f"{name} needs reduction 'mean' or 'sum', got {reduction!r}")
-    return _Distillation.apply(logits, values.detach(), indices, log_rest, weights, _check_temperature(name, temperature),
-                               float(scale), reduction == "mean")
+    return distill_op()(logits, values.detach(), indices, log_rest, weights, _check_temperature(name, temperature),
+                        float(scale), reduction == "mean", _UNITS.get((logits.device, torch.float32)))
 
 
 def sample_tokens(
