@@ -887,7 +887,7 @@ __device__ __forceinline__ Drawn draw_from_chunks(const Row<T, THREADS> &row, co
 }
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) {
+__global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 4) void sample_kernel(SampleKernelArgs a) {
     using R = Row<T, THREADS>;
     constexpr int N = R::N;
     __shared__ Shared<THREADS, true> sh;
@@ -974,7 +974,10 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
         __syncthreads();
     };
     if (!(top_p < 1.f)) {
-        sum_chunks(w.m - 41.f / inverse, [&](float, float e, int, int, int, const words4 &) { return e >= min_p; });
+        if (min_p > 0.f)
+            sum_chunks(w.m - 41.f / inverse, [&](float, float e, int, int, int, const words4 &) { return e >= min_p; });
+        else
+            sum_chunks(w.m - 41.f / inverse, [](float, float, int, int, int, const words4 &) { return true; });
         return finish(draw_from_chunks(
             row, chunks, u,
             [&](float x, int) -> u64 {
@@ -1066,9 +1069,9 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
 // Threads for a row: its pieces fill a slab or a few, and the list holds four
 // times k. Many wide rows take fewer, so that several fit a CU and one's
 // reductions hide behind another's stream.
-int threads_for(const LogitRows &x, int per_load, int k) {
+int threads_for(const LogitRows &x, int per_load, int k, int most, int many) {
     const int pieces = (x.vocab + per_load - 1) / per_load;
-    const int by_row = pieces <= 64 ? 64 : pieces <= 2048 || x.rows >= 512 ? 256 : pieces <= 8192 ? 512 : 1024;
+    const int by_row = pieces <= 64 ? 64 : pieces <= 2048 ? 256 : x.rows >= 512 ? many : min(most, pieces <= 8192 ? 512 : 1024);
     return max(by_row, k <= 64 ? 64 : k <= 256 ? 256 : k <= 512 ? 512 : 1024);
 }
 static_assert(TROPNN_MAX_VOCAB / (kWave * kSlab * kPerLoad<float>) <= kMaxChunks, "chunks of the widest row");
@@ -1092,7 +1095,7 @@ hipError_t launch_top_logits(const TopArgs &a, void *, hipStream_t stream) {
     const TopKernelArgs k{a.x.p, a.x.stride, a.x.vocab, a.k, a.temperature, a.values, a.indices, a.log_rest};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(threads_for(a.x, kPerLoad<T>, a.k), [&](auto threads) {
+        return with_threads(threads_for(a.x, kPerLoad<T>, a.k, 512, 256), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((top_logits_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
@@ -1108,7 +1111,7 @@ hipError_t launch_sample(const SampleArgs &a, void *, hipStream_t stream) {
                              a.temperature, a.top_p, a.min_p, a.top_k, a.tokens, a.log_probs};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(threads_for(a.x, kPerLoad<T>, a.top_ks ? 1 : max(a.top_k, 1)), [&](auto threads) {
+        return with_threads(threads_for(a.x, kPerLoad<T>, a.top_ks ? 1 : max(a.top_k, 1), 1024, 512), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((sample_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
