@@ -563,14 +563,11 @@ hipError_t launch_rows(K kernel, int threads, int64_t grid, int lds, const Disti
     return hipGetLastError();
 }
 
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool GRAD>
 hipError_t launch_streamed(const DistillKernelArgs &k, hipStream_t stream) {
     const int lds = k.log_rest ? k.bitmap_words * 4 : 0;
-    if (k.grad)
-        return k.log_rest ? launch_rows(distill_stream_kernel<T, THREADS, true, true>, THREADS, k.rows, lds, k, stream)
-                          : launch_rows(distill_stream_kernel<T, THREADS, false, true>, THREADS, k.rows, lds, k, stream);
-    return k.log_rest ? launch_rows(distill_stream_kernel<T, THREADS, true, false>, THREADS, k.rows, lds, k, stream)
-                      : launch_rows(distill_stream_kernel<T, THREADS, false, false>, THREADS, k.rows, lds, k, stream);
+    return k.log_rest ? launch_rows(distill_stream_kernel<T, THREADS, true, GRAD>, THREADS, k.rows, lds, k, stream)
+                      : launch_rows(distill_stream_kernel<T, THREADS, false, GRAD>, THREADS, k.rows, lds, k, stream);
 }
 
 constexpr int kCus = 256;
@@ -596,7 +593,8 @@ hipError_t launch_held(const DistillKernelArgs &k, hipStream_t stream) {
 template <typename T>
 hipError_t launch_by_width(const DistillKernelArgs &k, hipStream_t stream) {
     const int pieces = (k.vocab + kPerLoad<T> - 1) / kPerLoad<T>;
-    if (k.grad && k.vocab >= kPerLoad<T>) {
+    if (k.grad) {
+        if (k.vocab < kPerLoad<T>) return launch_streamed<T, 64, true>(k, stream);  // no whole piece to hold
         if (pieces <= 128) return launch_held<T, 64, 2, 16>(k, stream);
         if (pieces <= 256) return launch_held<T, 64, 4, 16>(k, stream);
         if (pieces <= 512) return launch_held<T, 64, 8, 16>(k, stream);
@@ -605,10 +603,11 @@ hipError_t launch_by_width(const DistillKernelArgs &k, hipStream_t stream) {
         if (pieces <= 4096) return launch_held<T, 512, 8, 2>(k, stream);
         if (pieces <= 8192) return launch_held<T, 512, 16, 2>(k, stream);
         if (pieces <= 16384) return launch_held<T, 1024, 16, 1>(k, stream);
+        return launch_streamed<T, 1024, true>(k, stream);
     }
-    if (pieces <= 256) return launch_streamed<T, 64>(k, stream);
-    if (!k.grad && (pieces <= 4096 || k.rows >= 4 * kCus)) return launch_streamed<T, 256>(k, stream);
-    return launch_streamed<T, 1024>(k, stream);
+    if (pieces <= 256) return launch_streamed<T, 64, false>(k, stream);
+    if (pieces <= 4096 || k.rows >= 4 * kCus) return launch_streamed<T, 256, false>(k, stream);
+    return launch_streamed<T, 1024, false>(k, stream);
 }
 
 }  // namespace

@@ -3,8 +3,6 @@
 // ordering logits and reducing over a workgroup.
 #pragma once
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -189,17 +187,14 @@ struct ExpSum {
     }
 };
 
-__device__ __forceinline__ ExpSum lane_join(ExpSum v, int distance, float c) {
-    ExpSum o;
-    o.m = __shfl_xor(v.m, distance, kWave);
-    o.s = __shfl_xor(v.s, distance, kWave);
-    v.join(o, c);
-    return v;
-}
-
 __device__ __forceinline__ ExpSum wave_join(ExpSum v, float c) {
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) v = lane_join(v, d, c);
+    for (int d = 1; d < kWave; d <<= 1) {
+        ExpSum o;
+        o.m = __shfl_xor(v.m, d, kWave);
+        o.s = __shfl_xor(v.s, d, kWave);
+        v.join(o, c);
+    }
     return v;
 }
 
@@ -236,8 +231,6 @@ __device__ __forceinline__ float wave_total(float v) {
 __device__ __forceinline__ float wave_most_of(float v) {
     return wave_fold(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
-
-__device__ __forceinline__ float wave_sum(float v) { return group_sum(v, kWave); }
 
 template <typename V>
 __device__ __forceinline__ V wave_add(V v) {

@@ -660,7 +660,7 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a)
         a.indices[r * a.k + j] = i;
         static_cast<T *>(a.values)[r * a.k + j] = row.x[i];
     }
-    sum = wave_sum(sum);
+    sum = wave_total(sum);
     if ((tid & (kWave - 1)) == 0) sh.wave_key[tid / kWave] = __builtin_bit_cast(uint32_t, sum);
     __syncthreads();
     sum = extra;
