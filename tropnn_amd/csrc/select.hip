@@ -14,10 +14,12 @@
 // whole row's: the weights are summed by exponent in LDS, which gives the mass
 // and the narrow range of logits in which the prefix ends. Rows that defeat
 // these (thousands of equal logits at the bound, rising rows) take the exact
-// search instead: a cut is found digit by digit, from the mass (a count, or the sampling weights as integers) of every
-// value of the key's next eight bits among the logits that share the digits
-// before (find_cut). Integer sums do not depend on their order, so neither
-// does a cut or a drawn token.
+// search instead: a cut is found digit by digit, from the mass (a count, or the
+// sampling weights as integers) of every value of the key's next eight bits
+// among the logits that share the digits before (find_cut). It reads the row
+// five times and more: 256 rows of 131072 bf16, 32 first of equal logits 531 us,
+// of random ones 23. Integer sums do not depend on their order, so neither does
+// a cut or a drawn token.
 #include "logits.hpp"
 
 namespace tropnn {
@@ -315,8 +317,8 @@ __device__ __forceinline__ int slots_for(int n) { return n <= 1 ? 1 : 1 << (32 -
 // Sorts the first n numbers of the list (all different), largest first. A
 // number's place is the count of larger ones; the threads share the counting.
 // n^2 / THREADS comparisons against broadcast reads beat the sorting network's
-// chain of LDS round trips (80 numbers, 512 threads: 5 us with the network)
-// until they are many.
+// chain of LDS round trips (80 numbers, 512 threads: 5 us with the network, 1
+// by counting) until they are many.
 template <typename SH>
 __device__ __forceinline__ void sort_list(int n, SH &sh) {
     constexpr int THREADS = SH::kThreads;
@@ -611,6 +613,14 @@ struct TopKernelArgs {
     float *log_rest;
 };
 
+// The row is read once, and the k entries once more (they are in the caches):
+// a row of 4096 x 131072 bf16, k = 64, costs its exponentials and comparisons
+// as much as its bytes: 215 us for 1.07 GB (5 TB/s) with the vector units 74 %
+// busy, where a reading rate of 6.7 TB/s would take 160. Of few rows, the chain
+// of the bound, the list and its sorting is left: 8 rows take 10 us of 1024
+// logits, 12 of 16384 and 15 of 65536. Exponentials are taken around the bound, known before
+// the stream begins, so no running maximum is carried: one product and
+// addition, one power of two and one addition a logit.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a) {
     constexpr int N = Row<T, THREADS>::N;
@@ -886,8 +896,20 @@ __device__ __forceinline__ Drawn draw_from_chunks(const Row<T, THREADS> &row, co
     return d;
 }
 
+// A row whose top_k fits the list is read once (collect) and drawn from the
+// sorted list: 24 us for 256 rows of 131072 bf16 (2.8 TB/s; the chain after the
+// stream is half of it). Any other row is read for its largest logit, and then
+// from the caches: once without top_p (29 us), where each wave's share of a slab
+// has its exact sum and the draw reads one such share again; with top_p (63 us)
+// once for the mass by exponent and once for the sums up to the cut. There
+// memory is done after 10 us and what bounds it are the additions to the
+// histogram in LDS (19 us: neighbours in a wave often hit one bin and go one by
+// one) and the second pass's exponentials and f64 sums (18 us). Holding the row
+// in registers between the passes spills or leaves one workgroup a CU (78 us).
+// The larger of the two ways a top_k can go: by the list up to a logit a thread,
+// 80 us for 1024 of a row at its widest, 50 for 512, 24 for 50; by search 205.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 4) void sample_kernel(SampleKernelArgs a) {
+__global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) {
     using R = Row<T, THREADS>;
     constexpr int N = R::N;
     __shared__ Shared<THREADS, true> sh;
@@ -1066,20 +1088,36 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 4) void sample_kernel(
         sh));
 }
 
-// Threads for a row: its pieces fill a slab or a few, and the list holds four
-// times k. Many wide rows take fewer, so that several fit a CU and one's
-// reductions hide behind another's stream.
-int threads_for(const LogitRows &x, int per_load, int k, int most, int many) {
-    const int pieces = (x.vocab + per_load - 1) / per_load;
-    const int by_row = pieces <= 64 ? 64 : pieces <= 2048 ? 256 : x.rows >= 512 ? many : min(most, pieces <= 8192 ? 512 : 1024);
-    return max(by_row, k <= 64 ? 64 : k <= 256 ? 256 : k <= 512 ? 512 : 1024);
+// Threads for a row, at least a quarter of what the list holds for each of the
+// k. Many rows take few threads, so that several workgroups fit a CU and one's
+// reductions, chains of LDS round trips that no more threads shorten, hide
+// behind another's stream; few rows take as many as shorten the stream.
+constexpr int kManyRows = 512;
+int threads_for_list(int k) { return k <= 64 ? 64 : k <= 256 ? 256 : k <= 512 ? 512 : 1024; }
+
+// bf16, k = 32, us: 8192 x 1024 64 threads 50, 256 61, 512 161; 4096 x 4096 36,
+// 40, 93; 1024 x 16384 30, 17, 28; 1024 x 131072 92, 56, 61; of 8 rows, 1024
+// classes 14.1, 10.5, 11.2; 16384 23, 11.6, 12.0; 131072 77, 26.9, 20.1 and 20.8
+// with 1024.
+int top_threads(const LogitRows &x, int pieces, int k) {
+    const int by_row = x.rows >= kManyRows ? (pieces <= 512 ? 64 : 256) : pieces <= 2048 ? 256 : 512;
+    return max(by_row, threads_for_list(k));
+}
+
+// bf16, us, untruncated / top_p 0.9 / top_k 50: 4096 x 512 64 threads 61 / 98 /
+// 54, 256 32 / 55 / 39, 512 54 / 90 / 76; 1024 x 32768 256 31 / 59 / 22, 512 28 /
+// 56 / 32, 1024 39 / 84 / 53; of 8 rows, 1024 classes 256 9.0 / 15.6 / 10.3, 512
+// 7.4 / 12.2 / 10.3, 1024 8.3 / 13.0 / 12.0; 32768 512 9.2 / 19.7 / 11.8, 1024
+// 9.4 / 20.8 / 12.9; 65536 512 12.8 / 31.1 / 14.0, 1024 11.7 / 27.3 / 14.7.
+int sample_threads(const LogitRows &x, int pieces, int top_k) {
+    const int by_row = x.rows >= kManyRows ? (pieces <= 2048 || top_k > 0 ? 256 : 512) : pieces <= 4096 ? 512 : 1024;
+    return max(by_row, threads_for_list(top_k));
 }
 static_assert(TROPNN_MAX_VOCAB / (kWave * kSlab * kPerLoad<float>) <= kMaxChunks, "chunks of the widest row");
 
 template <typename F>
 hipError_t with_threads(int threads, F &&f) {
     switch (threads) {
-        case 64: return f(std::integral_constant<int, 64>{});
         case 256: return f(std::integral_constant<int, 256>{});
         case 512: return f(std::integral_constant<int, 512>{});
         default: return f(std::integral_constant<int, 1024>{});
@@ -1095,11 +1133,13 @@ hipError_t launch_top_logits(const TopArgs &a, void *, hipStream_t stream) {
     const TopKernelArgs k{a.x.p, a.x.stride, a.x.vocab, a.k, a.temperature, a.values, a.indices, a.log_rest};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(threads_for(a.x, kPerLoad<T>, a.k, 512, 256), [&](auto threads) {
+        auto with = [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((top_logits_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
-        });
+        };
+        const int threads = top_threads(a.x, (a.x.vocab + kPerLoad<T> - 1) / kPerLoad<T>, a.k);
+        return threads == 64 ? with(std::integral_constant<int, 64>{}) : with_threads(threads, with);
     });
 }
 
@@ -1111,7 +1151,8 @@ hipError_t launch_sample(const SampleArgs &a, void *, hipStream_t stream) {
                              a.temperature, a.top_p, a.min_p, a.top_k, a.tokens, a.log_probs};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_threads(threads_for(a.x, kPerLoad<T>, a.top_ks ? 1 : max(a.top_k, 1), 1024, 512), [&](auto threads) {
+        const int pieces = (a.x.vocab + kPerLoad<T> - 1) / kPerLoad<T>, top_k = a.top_ks ? 0 : a.top_k;
+        return with_threads(sample_threads(a.x, pieces, top_k), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
             hipLaunchKernelGGL((sample_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
             return hipGetLastError();
