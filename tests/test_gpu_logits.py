@@ -619,3 +619,23 @@ def test_refusals():
         sample_tokens(x, u, top_k=torch.ones(3, device=DEV))
     with pytest.raises(ValueError, match="temperature"):
         sample_tokens(x, u, temperature=torch.ones(2, device=DEV))
+
+
+def test_more_rows_than_one_grid_takes():
+    """2^21 + 3 rows of three classes: launched in two grids, each row answered.
+    Sums of 2^21 losses are f64 within and one f32 at the end: REL covers them."""
+    rows, gen = (1 << 21) + 3, torch.Generator().manual_seed(77)
+    x = torch.randn(rows, 3, generator=gen)
+    teacher = torch.randn(rows, 3, generator=gen)
+    got = top_logits(teacher.to(DEV), 3)
+    _, indices = order_of(teacher)
+    assert torch.equal(got.indices.cpu(), indices)
+    drawn = sample_tokens(x.to(DEV), torch.zeros(rows, device=DEV), temperature=0.0)
+    assert torch.equal(drawn.tokens.cpu(), order_of(x)[1][:, 0])
+    logits = x.to(DEV).requires_grad_()
+    loss = distillation_loss(logits, got.values, got.indices, reduction="sum")
+    loss.backward()
+    log_q, log_p = torch.log_softmax(x.double(), -1), torch.log_softmax(teacher.double(), -1)
+    want = (log_p.exp() * (log_p - log_q)).sum()
+    assert abs(float(loss.detach()) - float(want)) <= 4 * REL * float(want)
+    assert float((logits.grad.cpu().double() - (log_q.exp() - log_p.exp())).abs().max()) <= REL

@@ -17,7 +17,7 @@ namespace {
 
 struct DistillKernelArgs {
     const void *x;
-    int64_t rows, stride;
+    int64_t rows, stride, first_row;  // first_row: of the streaming kernel's grid
     int vocab, k, values_dtype;
     const void *values;
     const int64_t *indices;
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(THREADS) void distill_stream_kernel(DistillKernelAr
     __shared__ ListSums lists[kWaves];
     const W k(args);
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
+    const int64_t row = args.first_row + blockIdx.x;
     const float norm = args.norm ? *args.norm : args.norm_value, weight = k.weight(row);
     if (weight == 0.f) {
         if (GRAD) k.store_zeros(row, tid);
@@ -562,29 +562,38 @@ __global__ __launch_bounds__(256) void scale_in_place_kernel(T *x, int64_t n, co
     }
 }
 
-template <typename K>
-hipError_t launch_rows(K kernel, int threads, int64_t grid, int lds, const DistillKernelArgs &k, hipStream_t stream) {
+template <typename T, int THREADS, bool REST, bool GRAD>
+hipError_t launch_stream(DistillKernelArgs k, hipStream_t stream) {
+    const auto kernel = distill_stream_kernel<T, THREADS, REST, GRAD>;
+    const int lds = REST ? k.bitmap_words * 4 : 0;
     if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void *>(kernel), lds); e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(threads), lds, stream, k);
-    return hipGetLastError();
+    return by_grids(k.rows, [&](int64_t first, uint32_t rows) {
+        k.first_row = first;
+        hipLaunchKernelGGL(kernel, dim3(rows), dim3(THREADS), lds, stream, k);
+    });
 }
 
 template <typename T, int THREADS, bool GRAD>
 hipError_t launch_streamed(const DistillKernelArgs &k, hipStream_t stream) {
-    const int lds = k.log_rest ? k.bitmap_words * 4 : 0;
-    return k.log_rest ? launch_rows(distill_stream_kernel<T, THREADS, true, GRAD>, THREADS, k.rows, lds, k, stream)
-                      : launch_rows(distill_stream_kernel<T, THREADS, false, GRAD>, THREADS, k.rows, lds, k, stream);
+    return k.log_rest ? launch_stream<T, THREADS, true, GRAD>(k, stream) : launch_stream<T, THREADS, false, GRAD>(k, stream);
 }
 
 constexpr int kCus = 256;
 
+template <typename T, int THREADS, int HOLD, bool REST>
+hipError_t launch_hold(const DistillKernelArgs &k, int64_t grid, hipStream_t stream) {
+    const auto kernel = distill_held_kernel<T, THREADS, HOLD, REST>;
+    const int lds = REST ? 2 * k.bitmap_words * 4 : 0;
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void *>(kernel), lds); e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(THREADS), lds, stream, k);
+    return hipGetLastError();
+}
+
 // WGS workgroups of a CU share the rows.
 template <typename T, int THREADS, int HOLD, int WGS>
 hipError_t launch_held(const DistillKernelArgs &k, hipStream_t stream) {
-    const int lds = k.log_rest ? 2 * k.bitmap_words * 4 : 0;
     const int64_t grid = k.rows < kCus * WGS ? k.rows : kCus * WGS;
-    return k.log_rest ? launch_rows(distill_held_kernel<T, THREADS, HOLD, true>, THREADS, grid, lds, k, stream)
-                      : launch_rows(distill_held_kernel<T, THREADS, HOLD, false>, THREADS, grid, lds, k, stream);
+    return k.log_rest ? launch_hold<T, THREADS, HOLD, true>(k, grid, stream) : launch_hold<T, THREADS, HOLD, false>(k, grid, stream);
 }
 
 // The kernel for rows of `pieces` pieces. With gradient, the row is held
@@ -624,7 +633,7 @@ size_t distill_workspace(const LogitRows &x, int, bool) { return 16 + sizeof(flo
 hipError_t launch_distill(const DistillArgs &a, void *workspace, hipStream_t stream) {
     float *norm = static_cast<float *>(workspace), *row_loss = norm + 4;
     const bool sum_weights = a.mean && a.weights;
-    DistillKernelArgs k{a.x.p, a.x.rows, a.x.stride, a.x.vocab, a.k, a.values_dtype, a.values, a.indices, a.log_rest, a.weights,
+    DistillKernelArgs k{a.x.p, a.x.rows, a.x.stride, 0, a.x.vocab, a.k, a.values_dtype, a.values, a.indices, a.log_rest, a.weights,
                         sum_weights ? norm : nullptr, a.mean ? static_cast<float>(a.x.rows) : 1.f, a.temperature,
                         a.scale, row_loss, a.grad, 0};
     if (sum_weights) {

@@ -70,6 +70,18 @@ auto with_logit_type(int dtype, F &&f) {
     return f(__bf16{});
 }
 
+// A launch of a workgroup per row, in as many grids as the runtime's limit of
+// 2^32 threads a grid asks for: launch(first row, rows).
+template <typename F>
+hipError_t by_grids(int64_t rows, F &&launch) {
+    constexpr int64_t kMost = 1 << 21;  // of up to 1024 threads
+    for (int64_t first = 0; first < rows; first += kMost) {
+        launch(first, static_cast<uint32_t>(rows - first < kMost ? rows - first : kMost));
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 #if defined(__HIPCC__)
 
 constexpr float kLog2e = 1.44269504088896340736f;

@@ -605,7 +605,7 @@ __device__ __forceinline__ int collect(const Row<T, THREADS> &row, int k, SH &sh
 
 struct TopKernelArgs {
     const void *x;
-    int64_t stride;
+    int64_t stride, first_row;
     int vocab, k;
     float temperature;
     void *values;
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a)
     constexpr int N = Row<T, THREADS>::N;
     __shared__ Shared<THREADS, false> sh;
     const int tid = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int64_t r = a.first_row + blockIdx.x;
     const Row<T, THREADS> row{static_cast<const T *>(a.x) + r * a.stride, a.vocab};
     const float c = kLog2e / a.temperature;
 
@@ -710,7 +710,7 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a)
 
 struct SampleKernelArgs {
     const void *x;
-    int64_t stride;
+    int64_t stride, first_row;
     int vocab;
     const float *uniforms, *temperatures, *top_ps, *min_ps;
     const int32_t *top_ks;
@@ -915,7 +915,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
     __shared__ Shared<THREADS, true> sh;
     __shared__ u64 chunks[kMaxChunks];
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
-    const int64_t r = blockIdx.x;
+    const int64_t r = a.first_row + blockIdx.x;
     const R row{static_cast<const T *>(a.x) + r * a.stride, a.vocab};
     const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
     const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
@@ -1130,13 +1130,15 @@ size_t top_logits_workspace(const LogitRows &, int) { return 0; }
 
 hipError_t launch_top_logits(const TopArgs &a, void *, hipStream_t stream) {
     if (a.x.rows == 0) return hipSuccess;
-    const TopKernelArgs k{a.x.p, a.x.stride, a.x.vocab, a.k, a.temperature, a.values, a.indices, a.log_rest};
+    TopKernelArgs k{a.x.p, a.x.stride, 0, a.x.vocab, a.k, a.temperature, a.values, a.indices, a.log_rest};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
         auto with = [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
-            hipLaunchKernelGGL((top_logits_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
-            return hipGetLastError();
+            return by_grids(a.x.rows, [&](int64_t first, uint32_t rows) {
+                k.first_row = first;
+                hipLaunchKernelGGL((top_logits_kernel<T, kThreads>), dim3(rows), dim3(kThreads), 0, stream, k);
+            });
         };
         const int threads = top_threads(a.x, (a.x.vocab + kPerLoad<T> - 1) / kPerLoad<T>, a.k);
         return threads == 64 ? with(std::integral_constant<int, 64>{}) : with_threads(threads, with);
@@ -1147,15 +1149,17 @@ size_t sample_workspace(const LogitRows &) { return 0; }
 
 hipError_t launch_sample(const SampleArgs &a, void *, hipStream_t stream) {
     if (a.x.rows == 0) return hipSuccess;
-    const SampleKernelArgs k{a.x.p, a.x.stride, a.x.vocab, a.uniforms, a.temperatures, a.top_ps, a.min_ps, a.top_ks,
+    SampleKernelArgs k{a.x.p, a.x.stride, 0, a.x.vocab, a.uniforms, a.temperatures, a.top_ps, a.min_ps, a.top_ks,
                              a.temperature, a.top_p, a.min_p, a.top_k, a.tokens, a.log_probs};
     return with_logit_type(a.x.dtype, [&](auto t) {
         using T = decltype(t);
         const int pieces = (a.x.vocab + kPerLoad<T> - 1) / kPerLoad<T>, top_k = a.top_ks ? 0 : a.top_k;
         return with_threads(sample_threads(a.x, pieces, top_k), [&](auto threads) {
             constexpr int kThreads = decltype(threads)::value;
-            hipLaunchKernelGGL((sample_kernel<T, kThreads>), dim3(static_cast<uint32_t>(a.x.rows)), dim3(kThreads), 0, stream, k);
-            return hipGetLastError();
+            return by_grids(a.x.rows, [&](int64_t first, uint32_t rows) {
+                k.first_row = first;
+                hipLaunchKernelGGL((sample_kernel<T, kThreads>), dim3(rows), dim3(kThreads), 0, stream, k);
+            });
         });
     });
 }
