@@ -639,3 +639,14 @@ def test_more_rows_than_one_grid_takes():
     want = (log_p.exp() * (log_p - log_q)).sum()
     assert abs(float(loss.detach()) - float(want)) <= 4 * REL * float(want)
     assert float((logits.grad.cpu().double() - (log_q.exp() - log_p.exp())).abs().max()) <= REL
+
+
+@pytest.mark.parametrize("levels", [3, 40, 700, 100000])
+@pytest.mark.parametrize("vocab,k", [(700, 300), (5000, 257), (5000, 900), (40000, 1024)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_lists_of_more_and_fewer_equal_logits(levels, vocab, k, dtype):
+    gen = torch.Generator().manual_seed(levels + vocab + k)
+    x = (torch.randint(0, levels, (5, vocab), generator=gen).double() / levels * 12 - 4).to(dtype)
+    x[3] = x[3].sort().values  # rising
+    x[4] = x[4].sort(descending=True).values
+    check_top(x.to(DEV), k)

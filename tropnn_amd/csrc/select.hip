@@ -27,10 +27,13 @@ namespace {
 
 constexpr int kBins = 256;
 constexpr int kSlab = 8;        // pieces of a thread that are in flight together
-constexpr int kKeyBins = 2048;  // of keys, by their distance from the largest
+constexpr int kKeyBinBits = 11;
+constexpr int kKeyBins = 1 << kKeyBinBits;  // of keys, by their distance from the largest
 constexpr int kKeyShift = 15;   // 2^15 keys a bin, 256 bins an octave
 constexpr int kMassBins = 2048; // of a row's weights, by exponent
-constexpr int kRanked = 1024;   // logits sorted by counting
+constexpr int kRanked = 256;    // logits sorted by counting all of them
+constexpr uint32_t kCrowd = 64; // of a bin, where they are sorted by bins
+constexpr uint32_t kSteps = 256;
 constexpr int kMaxChunks = 512; // a wave's share of a slab, in the widest row
 constexpr float kFixed = 1099511627776.f;  // 2^40: sampling weights are multiples of 2^-40
 
@@ -93,6 +96,10 @@ struct Row {
     static constexpr int kSlabLogits = THREADS * kSlab * N;
     const T *x;
     int n;
+
+    // Different keys of the type differ by 2^kKeyStep at least.
+    static constexpr int kKeyStep = sizeof(T) == 4 ? 0 : __is_same(T, __bf16) ? 16 : 13;
+    __device__ __forceinline__ int index_bits() const { return n > 1 ? 32 - __builtin_clz(n - 1) : 0; }
 
     __device__ __forceinline__ int slabs() const { return (n + kSlabLogits - 1) / kSlabLogits; }
 
@@ -314,33 +321,120 @@ __device__ __forceinline__ void sort_down(u64 *v, int n) {
 
 __device__ __forceinline__ int slots_for(int n) { return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)); }
 
-// Sorts the first n numbers of the list (all different), largest first. A
-// number's place is the count of larger ones; the threads share the counting.
-// n^2 / THREADS comparisons against broadcast reads beat the sorting network's
-// chain of LDS round trips (80 numbers, 512 threads: 5 us with the network, 1
-// by counting) until they are many.
+// Sorts the first n numbers of the list (all different), largest first.
+//
+// Few: a number's place is the count of larger ones; the threads share the
+// counting, n^2 / THREADS comparisons against broadcast reads (80 numbers, 512
+// threads: 1 us, 5 with the sorting network's chain of LDS round trips).
+// More: their upper words are counted in bins that share out their range; a
+// number's place is the count of the bins before and of the larger ones of its
+// own bin. 16-bit logits take few different keys, 2^step apart at least; where
+// the list has at most kSteps of them, each has bins of its own that share out
+// the places' indices (below 2^bits). Only where a bin is crowded all the same,
+// the network sorts. 500 of a row, 256 threads: 2.6 us, 9.4 with the network;
+// 1024, 1024 threads: 7.6, 20 by counting.
 template <typename SH>
-__device__ __forceinline__ void sort_list(int n, SH &sh) {
-    constexpr int THREADS = SH::kThreads;
+__device__ __forceinline__ void sort_list(int n, SH &sh, int step, int bits) {
+    constexpr int THREADS = SH::kThreads, kEach = kList<THREADS> / THREADS, kOwn = kKeyBins / THREADS;
     const int tid = threadIdx.x, slots = slots_for(max(n, kWave));
     __syncthreads();
-    if (n > kRanked || slots > THREADS) {
+    if (slots <= min(kRanked, THREADS)) {
+        const int i = tid & (slots - 1), part = tid / slots, parts = THREADS / slots;
+        const int per = (n + parts - 1) / parts, to = min(n, (part + 1) * per);
+        const u64 v = i < n ? sh.list[i] : 0;
+        if (part == 0) sh.ranks[i] = 0;
+        uint32_t rank = 0;
+#pragma unroll 4
+        for (int j = part * per; j < to; ++j) rank += sh.list[j] > v;
+        __syncthreads();
+        if (i < n && rank) atomicAdd(&sh.ranks[i], rank);
+        __syncthreads();
+        if (part == 0 && i < n) sh.list[min(static_cast<int>(sh.ranks[i]), n - 1)] = v;
+        __syncthreads();
+        return;
+    }
+    const int lane = tid & (kWave - 1), wave = tid / kWave;
+    u64 v[kEach];
+    uint32_t most = 0, least = 0;  // the least one's complement
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int j = tid + e * THREADS;
+        v[e] = j < n ? sh.list[j] : 0;
+        if (j < n) {
+            most = max(most, place_key(v[e]));
+            least = max(least, ~place_key(v[e]));
+        }
+    }
+    most = wave_max(most);
+    least = wave_max(least);
+    if (lane == 0) sh.wave[wave] = static_cast<u64>(most) << 32 | least;
+    for (int b = tid; b < kKeyBins; b += THREADS) sh.key_counts[b] = 0;
+    if (tid == 0) sh.bound = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / kWave; ++w) {
+        most = max(most, place_key(sh.wave[w]));
+        least = max(least, static_cast<uint32_t>(sh.wave[w]));
+    }
+    const uint32_t span = most - ~least;
+    const int shift = span < kKeyBins ? 0 : 21 - __builtin_clz(span);  // span >> shift < kKeyBins
+    const bool stepped = (span >> step) < kSteps;
+    const int each = kKeyBinBits - (span >> step ? 32 - __builtin_clz(span >> step) : 0);  // log2 of a key's own bins
+    const int index_shift = max(bits - each, 0);
+    auto bin_of = [&](u64 p) {
+        const uint32_t below = most - place_key(p);
+        return min(stepped ? (below >> step) << each | (~static_cast<uint32_t>(p) >> index_shift) : below >> shift,
+                   static_cast<uint32_t>(kKeyBins - 1));
+    };
+    uint32_t before[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (tid + e * THREADS < n) before[e] = atomicAdd(&sh.key_counts[bin_of(v[e])], 1u);
+    __syncthreads();
+    uint32_t count[kOwn], own = 0, crowd = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        count[j] = sh.key_counts[tid * kOwn + j];
+        own += count[j];
+        crowd = max(crowd, count[j]);
+    }
+    const uint32_t upto = wave_scan(own);
+    if (lane == kWave - 1) sh.wave_key[wave] = upto;
+    if (crowd > kCrowd) sh.bound = 1;
+    __syncthreads();
+    if (sh.bound) {
         const int padded = slots_for(n);
         for (int i = n + tid; i < padded; i += THREADS) sh.list[i] = 0;
         sort_down<THREADS>(sh.list, padded);
         return;
     }
-    const int i = tid & (slots - 1), part = tid / slots, parts = THREADS / slots;
-    const int per = (n + parts - 1) / parts, to = min(n, (part + 1) * per);
-    const u64 v = i < n ? sh.list[i] : 0;
-    if (part == 0) sh.ranks[i] = 0;
-    uint32_t rank = 0;
-#pragma unroll 4
-    for (int j = part * per; j < to; ++j) rank += sh.list[j] > v;
+    uint32_t from = upto - own;
+#pragma unroll
+    for (int w = 0; w < THREADS / kWave; ++w) from += w < wave ? sh.wave_key[w] : 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        sh.key_counts[tid * kOwn + j] = from;
+        from += count[j];
+    }
     __syncthreads();
-    if (i < n && rank) atomicAdd(&sh.ranks[i], rank);
+    // bin by bin
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (tid + e * THREADS < n) sh.list[min(sh.key_counts[bin_of(v[e])] + before[e], static_cast<uint32_t>(n - 1))] = v[e];
     __syncthreads();
-    if (part == 0 && i < n) sh.list[min(static_cast<int>(sh.ranks[i]), n - 1)] = v;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if (tid + e * THREADS < n) {
+            const uint32_t bin = bin_of(v[e]), first = sh.key_counts[bin];
+            const uint32_t end = bin + 1 < kKeyBins ? sh.key_counts[bin + 1] : static_cast<uint32_t>(n);
+            before[e] = first;
+            for (uint32_t j = first; j < end; ++j) before[e] += sh.list[j] > v[e];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (tid + e * THREADS < n) sh.list[min(before[e], static_cast<uint32_t>(n - 1))] = v[e];
     __syncthreads();
 }
 
@@ -660,9 +754,9 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a)
                 if (at < kList<THREADS>) sh.list[at] = p;
             }
         });
-        sort_list(a.k, sh);
+        sort_list(a.k, sh, row.kKeyStep, row.index_bits());
     } else {
-        sort_list(n, sh);
+        sort_list(n, sh, row.kKeyStep, row.index_bits());
         for (int j = a.k + tid; j < n; j += THREADS) rest.join(ExpSum::of(key_logit(place_key(sh.list[j]))), c);
     }
     for (int j = tid; j < a.k; j += THREADS) {
@@ -819,7 +913,7 @@ __device__ __forceinline__ Drawn draw_from_list(int n, const Weights &w, float t
     }
     // by index: halves swapped, the larger complement of the index is first
     for (int i = tid; i < kept; i += THREADS) sh.list[i] = sh.list[i] << 32 | sh.list[i] >> 32;
-    sort_list(kept, sh);
+    sort_list(kept, sh, 0, 32);
     if (tid < kWave) {
         const u64 target = target_of(u, d.sum);
         const int per = (kept + kWave - 1) / kWave, from = tid * per, to = min(kept, from + per);
@@ -951,7 +1045,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
             [](const float (&)[N]) { return 0.f; });
         if (n == 0) return answer(-1, NAN);  // no logit above -inf
         if (n > 0) {
-            sort_list(n, sh);
+            sort_list(n, sh, row.kKeyStep, row.index_bits());
             const u64 top = sh.list[0];
             const Weights w{key_logit(place_key(top)), inverse};
             if (place_key(top) == kKeyNan || place_key(top) == kKeyNegInf) return answer(-1, NAN);
@@ -1061,7 +1155,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) 
                });
     const int n = sh.count;
     if (n > kList<THREADS>) return finish(draw_by_search(row, w, top_k, top_p, min_p, u, sh));
-    sort_list(n, sh);
+    sort_list(n, sh, row.kKeyStep, row.index_bits());
     const int per = (n + THREADS - 1) / THREADS, from = tid * per, to = min(n, from + per);
     own = 0;
     for (int j = from; j < to; ++j) own += w.fixed(key_logit(place_key(sh.list[j])));
