@@ -994,16 +994,18 @@ __device__ __forceinline__ Drawn draw_from_chunks(const Row<T, THREADS> &row, co
 // sorted list: 24 us for 256 rows of 131072 bf16 (2.8 TB/s; the chain after the
 // stream is half of it). Any other row is read for its largest logit, and then
 // from the caches: once without top_p (29 us), where each wave's share of a slab
-// has its exact sum and the draw reads one such share again; with top_p (63 us)
+// has its exact sum and the draw reads one such share again; with top_p (60 us)
 // once for the mass by exponent and once for the sums up to the cut. There
 // memory is done after 10 us and what bounds it are the additions to the
 // histogram in LDS (19 us: neighbours in a wave often hit one bin and go one by
 // one) and the second pass's exponentials and f64 sums (18 us). Holding the row
 // in registers between the passes spills or leaves one workgroup a CU (78 us).
 // The larger of the two ways a top_k can go: by the list up to a logit a thread,
-// 80 us for 1024 of a row at its widest, 50 for 512, 24 for 50; by search 205.
+// 41 us for 1024 of a row at its widest, 33 for 512, 24 for 50; by search 205.
+// Five workgroups of 256 threads fit a CU (LDS, and registers if no more than
+// 96): 8192 x 1024, top_p 0.9, 106 us, with four 125.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleKernelArgs a) {
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? 5 : 4) void sample_kernel(SampleKernelArgs a) {
     using R = Row<T, THREADS>;
     constexpr int N = R::N;
     __shared__ Shared<THREADS, true> sh;
