@@ -33,7 +33,7 @@ constexpr int kKeyShift = 15;   // 2^15 keys a bin, 256 bins an octave
 constexpr int kMassBins = 2048; // of a row's weights, by exponent
 constexpr int kRanked = 256;    // logits sorted by counting all of them
 constexpr uint32_t kCrowd = 64; // of a bin, where they are sorted by bins
-constexpr uint32_t kSteps = 256;
+constexpr uint32_t kSteps = 256; // different keys of a list sorted by key and index
 constexpr int kMaxChunks = 512; // a wave's share of a slab, in the widest row
 constexpr float kFixed = 1099511627776.f;  // 2^40: sampling weights are multiples of 2^-40
 
