@@ -650,3 +650,21 @@ def test_long_lists_of_more_and_fewer_equal_logits(levels, vocab, k, dtype):
     x[3] = x[3].sort().values  # rising
     x[4] = x[4].sort(descending=True).values
     check_top(x.to(DEV), k)
+
+
+@pytest.mark.parametrize("vocab", [7, 130, 5000, 40007])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_a_rows_answer_is_the_same_in_large_and_small_batches(vocab, dtype):
+    """Batches of 700 rows and of 50 take different numbers of threads a row;
+    lists and tokens are the same bits, log-masses within their bound."""
+    x, u = rows_of(700, vocab, dtype, vocab), torch.rand(700, generator=torch.Generator().manual_seed(1)).to(DEV)
+    part = slice(300, 350)
+    k = min(vocab, 40)
+    check_top(x, k)
+    small, large = top_logits(x[part], k), top_logits(x, k)
+    assert torch.equal(small.values, large.values[part]) and torch.equal(small.indices, large.indices[part])
+    for kw in ({}, dict(top_p=0.9), dict(top_k=50, min_p=0.02), dict(top_k=300, top_p=0.95), dict(temperature=0.0),
+               dict(temperature=3.0, top_p=0.6), dict(min_p=0.1)):
+        small, large = sample_tokens(x[part], u[part], **kw), sample_tokens(x, u, **kw)
+        assert torch.equal(small.tokens, large.tokens[part]), kw
+        assert torch.equal(small.log_probs, large.log_probs[part]), kw
