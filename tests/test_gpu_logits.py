@@ -668,3 +668,39 @@ def test_a_rows_answer_is_the_same_in_large_and_small_batches(vocab, dtype):
         small, large = sample_tokens(x[part], u[part], **kw), sample_tokens(x, u, **kw)
         assert torch.equal(small.tokens, large.tokens[part]), kw
         assert torch.equal(small.log_probs, large.log_probs[part]), kw
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("layout", [
+    "a new inner dimension", "inner dimension broadcast", "a new middle dimension", "two new dimensions",
+    "outer dimension broadcast", "both broadcast", "slice", "one of the inner dimension", "every second row", "classes apart",
+])
+def test_distillation_leading_dimensions_and_layouts(layout, dtype):
+    """Loss and gradient of logits in any layout are those of a contiguous copy."""
+    base = rows_of(4 * 6, 500, dtype, 1, pad=4).unflatten(0, (4, 6))
+    x = {
+        "a new inner dimension": lambda: base[:, 0][:, None].expand(4, 8, 500),
+        "inner dimension broadcast": lambda: base[:, :1].expand(4, 6, 500),
+        "a new middle dimension": lambda: base[:, None].expand(4, 3, 6, 500),
+        "two new dimensions": lambda: base[:, 0][:, None, None].expand(4, 2, 3, 500),
+        "outer dimension broadcast": lambda: base[:1].expand(4, 6, 500),
+        "both broadcast": lambda: base[:1, :1].expand(4, 6, 500),
+        "slice": lambda: base[..., 3:450],
+        "one of the inner dimension": lambda: base[:, 1],
+        "every second row": lambda: base[:, ::2],
+        "classes apart": lambda: base.transpose(1, 2).contiguous().transpose(1, 2),
+    }[layout]()
+    lead, vocab, k = x.shape[:-1], x.shape[-1], 7
+    values, indices, log_rest = (t.reshape(*lead, *t.shape[1:]) for t in make_record(x.numel() // vocab, vocab, k, 2, t=1.5))
+    weights = torch.linspace(0.0, 2.0, log_rest.numel(), device=DEV).reshape(lead)
+
+    def run(logits):
+        logits = logits.detach().requires_grad_(True)
+        loss = distillation_loss(logits, values, indices, log_rest, weights=weights, temperature=1.5)
+        loss.backward()
+        with torch.no_grad():
+            alone = distillation_loss(logits, values, indices, log_rest, weights=weights, temperature=1.5)
+        return loss.detach(), alone, logits.grad
+
+    assert all(torch.equal(a, b) for a, b in zip(run(x), run(x.contiguous())))
+    check_distill(x.contiguous(), values, indices, log_rest, weights, t=1.5)

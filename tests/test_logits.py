@@ -101,6 +101,52 @@ def test_as_rows_reads_slices_where_they_are():
     assert lh.as_rows(torch.zeros(0, 7))[1:3] == (0, 7)
 
 
+LAYOUTS = {
+    "contiguous": lambda x: x,
+    "one row": lambda x: x[0, 0],
+    "slice of the classes": lambda x: x[..., 5:25],
+    "one of the inner dimension": lambda x: x[:, 1],
+    "every second row": lambda x: x[:, ::2, :],
+    "every second of two": lambda x: x[:, :4:2, :],
+    "no common stride": lambda x: x[:, :3, :20],
+    "inner dimension broadcast": lambda x: x[:, :1].expand(4, 6, 40),
+    "inner dimension broadcast, a slice": lambda x: x[:, 2:3, 3:23].expand(4, 6, 20),
+    "outer dimension broadcast": lambda x: x[:1].expand(4, 6, 40),
+    "both broadcast": lambda x: x[:1, :1].expand(4, 6, 40),
+    "a new inner dimension": lambda x: x[:, 0][:, None].expand(4, 8, 40),
+    "a new middle dimension": lambda x: x[:, None].expand(4, 3, 6, 40),
+    "a new innermost of three": lambda x: x[:, :, None].expand(4, 6, 3, 40),
+    "two new dimensions": lambda x: x[:, 0][:, None, None].expand(4, 2, 3, 40),
+    "dimensions of one": lambda x: x[:, :1].unsqueeze(0),
+    "dimensions exchanged": lambda x: x.transpose(0, 1),
+    "classes apart": lambda x: x.transpose(1, 2),
+    "classes broadcast": lambda x: x[..., :1].expand(4, 6, 40),
+    "one class": lambda x: x[..., 7:8],
+    "one class, broadcast": lambda x: x[:, :1, 7:8].expand(4, 6, 1),
+    "no rows": lambda x: x[:0],
+    "no rows, broadcast": lambda x: x[:, :0],
+}
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_rows_are_read_inside_the_tensor_and_in_order(lib, layout):
+    """What the operators take as rows of logits, the Python functions' and the
+    autograd operator's, is the tensor's rows, and inside its memory."""
+    lh.distill_op()  # loads the operator library
+    base = torch.arange(4 * 6 * 40, dtype=torch.float32)
+    logits = LAYOUTS[layout](base.view(4, 6, 40))
+    for as_rows in (lh.as_rows, torch.ops.tropnn_hip.logit_rows):
+        t, rows, vocab, stride = as_rows(logits)
+        assert (rows, vocab) == (logits.numel() // logits.shape[-1], logits.shape[-1])
+        assert rows <= 1 or stride >= vocab
+        if rows == 0:
+            continue
+        end = t.storage_offset() + (rows - 1) * stride + vocab
+        assert end <= t.untyped_storage().nbytes() // 4, f"reads to element {end}"
+        read = torch.as_strided(t, (rows, vocab), (stride, 1), t.storage_offset())
+        assert torch.equal(read, logits.reshape(rows, vocab))
+
+
 def test_abi_refuses_bad_arguments(lib):
     p = 4096  # an address that is never read: every call here ends before a launch
     top = [2, 10, 10, p, F32, 3, 1.0, p, p, p, p, 1 << 20, None]

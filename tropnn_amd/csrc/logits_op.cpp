@@ -21,6 +21,7 @@
 #include <atomic>
 #include <cstdint>
 #include <optional>
+#include <tuple>
 
 #include "tropnn_hip_logits.h"
 
@@ -80,17 +81,17 @@ struct Rows {
 Rows as_rows(const Tensor &logits) {
     const int64_t dim = logits.dim(), vocab = logits.size(-1), rows = vocab > 0 ? logits.numel() / vocab : 0;
     if (logits.is_contiguous()) return {logits, rows, vocab, vocab};
-    int64_t stride = 0, span = 1;  // of a row; rows in the dimensions seen so far
+    std::optional<int64_t> stride;  // of a row, from the innermost dimension that has more than one
+    int64_t span = 1;               // rows in the dimensions seen so far
     bool even = logits.stride(-1) == 1 || vocab == 1;
     for (int64_t i = dim - 2; even && i >= 0; --i) {
         if (logits.size(i) == 1) continue;
-        if (stride == 0)
-            stride = logits.stride(i);
-        else
-            even = logits.stride(i) == stride * span;
+        if (!stride) stride = logits.stride(i);
+        // rows on top of each other (a broadcast dimension) are no rows of a matrix
+        even = *stride >= vocab && logits.stride(i) == *stride * span;
         span *= logits.size(i);
     }
-    if (even && (stride >= vocab || rows <= 1)) return {logits, rows, vocab, stride == 0 ? vocab : stride};
+    if (even) return {logits, rows, vocab, stride.value_or(vocab)};
     return {logits.contiguous(), rows, vocab, vocab};
 }
 
@@ -190,6 +191,11 @@ TORCH_LIBRARY_FRAGMENT(tropnn_hip, m) {
     m.def("bind_logits_abi(int distill, int distill_workspace_size, int scale_in_place, int last_error, "
           "int abi_version) -> ()",
           &bind_logits_abi);
+    // the layout that distill reads logits in, for any device: (tensor, rows, vocab, row stride)
+    m.def("logit_rows(Tensor logits) -> (Tensor, int, int, int)", [](const Tensor &logits) {
+        const Rows x = as_rows(logits);
+        return std::make_tuple(x.t, x.rows, x.vocab, x.stride);
+    });
     m.def("distill(Tensor logits, Tensor values, Tensor indices, Tensor? log_rest, Tensor? weights, "
           "float temperature, float scale, bool mean, Tensor? unit) -> Tensor",
           &distill);
