@@ -13,7 +13,7 @@
  *  - The library does not allocate: `workspace` holds at least the bytes the
  *    matching _workspace_size query returns for the same arguments (NULL is
  *    fine where that is 0), 16-byte aligned, contents irrelevant before and
- *    after the call.
+ *    after the call (but for tropnn_hip_distill_grad with `holds`).
  *  - Calls are asynchronous on `stream`, and can be captured in a HIP graph.
  *  - The order of a row's logits is: larger value first, NaN before every
  *    number, -0 equal to +0, equal values by ascending index.
@@ -75,9 +75,24 @@ int tropnn_hip_distill(int64_t rows, int64_t vocab, int64_t row_stride, const vo
                        void *workspace, size_t workspace_bytes, tropnn_stream_t stream);
 
 /*
+ * The chain rule's product of that gradient with the incoming one, factor[0]:
+ * grad = factor[0] * d loss / d logits, rounded once to `dtype`. The arguments
+ * are those of tropnn_hip_distill and `grad` is non-NULL; no loss is given.
+ * holds != 0: grad is what tropnn_hip_distill wrote for the same arguments and
+ * workspace that call's, neither touched since. Where factor[0] is 1, grad is
+ * then left alone. holds == 0: the contents of both are irrelevant.
+ */
+int tropnn_hip_distill_grad(int64_t rows, int64_t vocab, int64_t row_stride, const void *logits, int dtype, int64_t k,
+                            const void *values, int values_dtype, const int64_t *indices, const float *log_rest,
+                            const float *weights, float temperature, float scale, int mean, const float *factor,
+                            int holds, void *grad, void *workspace, size_t workspace_bytes, tropnn_stream_t stream);
+
+/*
  * x[i] *= factor[0] for n contiguous elements of TROPNN_LOGITS_*, nothing
  * where factor[0] is 1: the chain rule's product of a saved gradient with the
- * incoming one, which is usually 1.
+ * incoming one, which is usually 1. It rounds a second time, which in f32 is
+ * nothing; what 16 bits lost at a small scale (f16 has no number below 2^-24)
+ * no factor brings back, so such a gradient takes tropnn_hip_distill_grad.
  */
 int tropnn_hip_scale_in_place(int64_t n, void *x, int dtype, const float *factor, tropnn_stream_t stream);
 

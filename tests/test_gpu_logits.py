@@ -704,3 +704,99 @@ def test_distillation_leading_dimensions_and_layouts(layout, dtype):
 
     assert all(torch.equal(a, b) for a, b in zip(run(x), run(x.contiguous())))
     check_distill(x.contiguous(), values, indices, log_rest, weights, t=1.5)
+
+
+def distill_reference_by_rows(logits, values, indices, log_rest, weights, t=1.0):
+    """distill_reference for many rows: the same formulas in 64 bits, a few
+    hundred rows at a time, on the GPU. Loss, gradient and the bound of its
+    error before it is stored, of the weighted mean."""
+    rows, vocab = logits.shape
+    w_all = torch.ones(rows, dtype=torch.float64, device=DEV) if weights is None else weights.double()
+    total, loss, grads, bounds = w_all.sum(), 0.0, [], []
+    for part in torch.arange(rows).split(max(1, (1 << 23) // vocab)):
+        part = slice(int(part[0]), int(part[-1]) + 1)
+        at, w = indices[part], w_all[part, None]
+        here = at >= 0
+        used = here.any(1, keepdim=True) & (w != 0)
+        log_q = torch.log_softmax(logits[part].double() / t, 1)
+        teacher = (values[part].double() / t).masked_fill(~here, -math.inf)
+        if log_rest is not None:
+            teacher = torch.cat((teacher, log_rest[part, None].double()), 1)
+        log_p = torch.log_softmax(teacher, 1)
+        p = log_p.exp()
+        q, k = log_q.exp(), at.shape[1]
+        spread = torch.zeros(len(at), vocab + 1, dtype=torch.float64, device=DEV)  # p by class; the last column: none
+        spread.scatter_(1, torch.where(here, at, vocab), p[:, :k])
+        listed = torch.zeros_like(spread, dtype=torch.bool).scatter_(1, torch.where(here, at, vocab), True)[:, :vocab]
+        spread = torch.where(listed, spread[:, :vocab], 0.0)
+        terms = torch.where(here & (p[:, :k] > 0), p[:, :k] * (log_p[:, :k] - log_q.gather(1, at.clamp(min=0))), 0.0).sum(1)
+        ratio = torch.zeros(len(at), 1, dtype=torch.float64, device=DEV)
+        if log_rest is not None:
+            log_q0 = torch.logsumexp(log_q.masked_fill(listed, -math.inf), 1)
+            p0 = p[:, k]
+            terms += torch.where(p0 > 0, p0 * (log_p[:, k] - log_q0), 0.0)
+            ratio = torch.where(p0 > 0, p0 / log_q0.exp(), 0.0)[:, None]
+        loss += torch.where(used[:, 0], w[:, 0] * t * t * terms, 0.0).sum()
+        coef = t * w / total
+        g = torch.where(listed, q - spread, q * (1 - ratio))
+        b = torch.where(listed, q + spread, q * (1 + ratio))
+        grads.append(torch.where(used, coef * g, 0.0))
+        bounds.append(torch.where(used, REL * coef * b, 0.0))
+    return loss / total, torch.cat(grads), torch.cat(bounds)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rest", [True, False])
+@pytest.mark.parametrize("rows,vocab,k", [(4099, 300, 8), (4099, 5, 2), (700, 9000, 33)])
+def test_distillation_scaled_losses(rows, vocab, k, rest, dtype):
+    """A loss scaled against f16's underflow (a mean over thousands of rows has
+    gradients below its smallest number): the gradient is the formula's times
+    the scale, rounded once. A scale of one that the host does not know, and a
+    second backward through the same graph, too."""
+    logits = rows_of(rows, vocab, dtype, 3)
+    values, indices, log_rest = make_record(rows, vocab, k, 4, t=2.0, rest=rest)
+    weights = torch.rand(rows, generator=torch.Generator().manual_seed(5)).to(DEV)
+    weights[::7] = 0.0
+    want_loss, want, bound = distill_reference_by_rows(logits, values, indices, log_rest, weights, t=2.0)
+
+    def check(grad, factor):
+        off = (grad.double() - factor * want).abs() - (abs(factor) * bound + HALF_ULP[dtype] * (factor * want).abs() + SMALLEST[dtype])
+        assert (off <= 0).all(), (factor, off.max())
+
+    x = logits.detach().requires_grad_(True)
+    for factor in (65536.0, -0.375, 1.0):
+        loss = distillation_loss(x, values, indices, log_rest, weights=weights, temperature=2.0)
+        assert abs(float(loss.detach()) - float(want_loss)) <= 4 * REL * (1 + abs(float(want_loss)))
+        (first,) = torch.autograd.grad(factor * loss, x, retain_graph=True)
+        check(first, factor)
+        (second,) = torch.autograd.grad(loss, x, torch.tensor(2 * factor, device=DEV))
+        check(second, 2 * factor)
+        if factor == 1.0:
+            again = distillation_loss(x, values, indices, log_rest, weights=weights, temperature=2.0)
+            assert torch.equal(first, torch.autograd.grad(again, x, unit_gradient(again))[0])
+
+
+def test_distillation_scaled_loss_in_a_graph():
+    """The scaled 16-bit backward captured and replayed on new inputs."""
+    logits = rows_of(600, 700, F16, 1)
+    values, indices, log_rest = make_record(600, 700, 9, 2)
+    factor = torch.tensor(1024.0, device=DEV)
+    weights = torch.linspace(0.0, 1.0, 600, device=DEV)
+
+    def run():
+        x = logits.detach().requires_grad_(True)
+        loss = distillation_loss(x, values, indices, log_rest, weights=weights)
+        return torch.autograd.grad(loss, x, factor)[0]
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for rep in range(4):
+        logits.copy_(rows_of(600, 700, F16, 10 + rep))
+        factor.fill_((1024.0, 1.0, 0.5, 4096.0)[rep])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run()
+        _ = torch.ones(64, device=DEV).sum().item()
+        assert torch.equal(out, want), rep

@@ -206,3 +206,21 @@ def test_workspace_queries(lib):
     assert lib.tropnn_hip_distill_workspace_size(100, 0, F32, 8, 1) == 0 and "vocab" in error(lib)
     assert lib.tropnn_hip_top_logits_workspace_size(-1, 10, F32, 8) == 0 and "rows" in error(lib)
     assert lib.tropnn_hip_sample_workspace_size(4, 10, 7) == 0 and "dtype" in error(lib)
+
+
+def test_abi_refuses_bad_arguments_of_the_scaled_gradient(lib):
+    p = 4096  # an address that is never read: every call here ends before a launch
+    good = [2, 10, 10, p, BF16, 3, p, F16, p, p, p, 1.0, 1.0, 1, p, 1, p, p, 1 << 20, None]
+    fn = lib.tropnn_hip_distill_grad
+    for at, value, word, code in (
+        (0, -1, "rows", 1), (1, (1 << 20) + 1, "vocab", 2), (2, 9, "row_stride", 1), (3, None, "logits", 1),
+        (4, 3, "dtype", 1), (5, 0, "k must", 1), (5, 1025, "k=", 2), (6, None, "non-NULL", 1), (7, 5, "values_dtype", 1),
+        (8, p + 4, "aligned", 1), (11, 0.0, "temperature", 1), (14, None, "non-NULL", 1), (14, p + 2, "aligned", 1),
+        (16, None, "non-NULL", 1), (16, p + 1, "aligned", 1), (17, None, "workspace", 1), (18, 4, "workspace", 1),
+    ):
+        args = list(good)
+        args[at] = value
+        assert fn(*args) == code and word in error(lib), (at, value, error(lib))
+    none = list(good)
+    none[0], none[3] = 0, None
+    assert fn(*none) == 0

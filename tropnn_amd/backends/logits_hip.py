@@ -25,6 +25,7 @@ LOGITS_SYMBOLS = (
     "tropnn_hip_top_logits",
     "tropnn_hip_distill_workspace_size",
     "tropnn_hip_distill",
+    "tropnn_hip_distill_grad",
     "tropnn_hip_scale_in_place",
     "tropnn_hip_sample_workspace_size",
     "tropnn_hip_sample",
@@ -42,6 +43,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         ("tropnn_hip_top_logits", [i64, i64, i64, p, i, i64, f, p, p, p, p, sz, p], i),
         ("tropnn_hip_distill_workspace_size", [i64, i64, i, i64, i], sz),
         ("tropnn_hip_distill", [i64, i64, i64, p, i, i64, p, i, p, p, p, f, f, i, p, p, p, sz, p], i),
+        ("tropnn_hip_distill_grad", [i64, i64, i64, p, i, i64, p, i, p, p, p, f, f, i, p, i, p, p, sz, p], i),
         ("tropnn_hip_scale_in_place", [i64, p, i, p, p], i),
         ("tropnn_hip_sample_workspace_size", [i64, i64, i], sz),
         ("tropnn_hip_sample", [i64, i64, i64, p, i, p, p, f, p, i32, p, f, p, f, p, p, p, sz, p], i),
@@ -83,8 +85,8 @@ def distill_op() -> Any:
     _pairwise_op()  # loads the operator library
     with _LOCK:
         if _DISTILL_OP is None:
-            names = ("tropnn_hip_distill", "tropnn_hip_distill_workspace_size", "tropnn_hip_scale_in_place",
-                     "tropnn_hip_last_error")
+            names = ("tropnn_hip_distill", "tropnn_hip_distill_workspace_size", "tropnn_hip_distill_grad",
+                     "tropnn_hip_scale_in_place", "tropnn_hip_last_error")
             torch.ops.tropnn_hip.bind_logits_abi(
                 *(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), LOGITS_ABI_VERSION)
             _DISTILL_OP = torch.ops.tropnn_hip.distill.default

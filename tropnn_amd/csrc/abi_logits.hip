@@ -71,6 +71,25 @@ int check_workspace(const void *workspace, size_t bytes, size_t need) {
     return TROPNN_OK;
 }
 
+// What tropnn_hip_distill and tropnn_hip_distill_grad have in common; x is
+// filled in.
+int check_distill(int64_t rows, int64_t vocab, int64_t row_stride, const void *logits, int dtype, int64_t k,
+                  const void *values, int values_dtype, const int64_t *indices, const float *log_rest,
+                  const float *weights, float temperature, const void *grad, const void *workspace,
+                  size_t workspace_bytes, tropnn::LogitRows &x) {
+    if (int rc = check_rows(rows, vocab, row_stride, logits, dtype, x)) return rc;
+    if (int rc = check_top(k)) return rc;
+    if (int rc = check_temperature(temperature)) return rc;
+    if (int rc = check_type("values_dtype", values_dtype)) return rc;
+    if (rows > 0 && (!values || !indices))
+        return abi_fail(TROPNN_ERR_INVALID_ARGUMENT, "values and indices must be non-NULL");
+    if (misaligned(values, element_size(values_dtype)) || misaligned(indices, 8) || misaligned(log_rest, 4) ||
+        misaligned(weights, 4) || misaligned(grad, element_size(dtype)))
+        return abi_fail(TROPNN_ERR_INVALID_ARGUMENT,
+                        "values, indices, log_rest, weights and grad must be aligned to their elements");
+    return check_workspace(workspace, workspace_bytes, tropnn::distill_workspace(x, static_cast<int>(k), grad != nullptr));
+}
+
 int launched(const char *what, hipError_t e) { return e == hipSuccess ? abi_ok() : abi_hip_fail(what, e); }
 
 }  // namespace
@@ -116,23 +135,31 @@ int tropnn_hip_distill(int64_t rows, int64_t vocab, int64_t row_stride, const vo
                        const void *values, int values_dtype, const int64_t *indices, const float *log_rest,
                        const float *weights, float temperature, float scale, int mean, float *loss, void *grad,
                        void *workspace, size_t workspace_bytes, tropnn_stream_t stream) {
+    if (!loss) return abi_fail(TROPNN_ERR_INVALID_ARGUMENT, "loss must be non-NULL");
+    if (misaligned(loss, 4)) return abi_fail(TROPNN_ERR_INVALID_ARGUMENT, "loss must be aligned to its elements");
     tropnn::LogitRows x{};
-    if (int rc = check_rows(rows, vocab, row_stride, logits, dtype, x)) return rc;
-    if (int rc = check_top(k)) return rc;
-    if (int rc = check_temperature(temperature)) return rc;
-    if (int rc = check_type("values_dtype", values_dtype)) return rc;
-    if (!loss || (rows > 0 && (!values || !indices)))
-        return abi_fail(TROPNN_ERR_INVALID_ARGUMENT, "values, indices and loss must be non-NULL");
-    if (misaligned(values, element_size(values_dtype)) || misaligned(indices, 8) || misaligned(log_rest, 4) ||
-        misaligned(weights, 4) || misaligned(loss, 4) || misaligned(grad, element_size(dtype)))
-        return abi_fail(TROPNN_ERR_INVALID_ARGUMENT,
-                        "values, indices, log_rest, weights, loss and grad must be aligned to their elements");
-    if (int rc = check_workspace(workspace, workspace_bytes,
-                                 tropnn::distill_workspace(x, static_cast<int>(k), grad != nullptr)))
+    if (int rc = check_distill(rows, vocab, row_stride, logits, dtype, k, values, values_dtype, indices, log_rest, weights,
+                               temperature, grad, workspace, workspace_bytes, x))
         return rc;
     const tropnn::DistillArgs a{x, values, indices, log_rest, weights, static_cast<int>(k), values_dtype, mean != 0,
-                                temperature, scale, loss, grad};
+                                temperature, scale, loss, grad, nullptr, false};
     return launched("distillation launch", tropnn::launch_distill(a, workspace, static_cast<hipStream_t>(stream)));
+}
+
+int tropnn_hip_distill_grad(int64_t rows, int64_t vocab, int64_t row_stride, const void *logits, int dtype, int64_t k,
+                            const void *values, int values_dtype, const int64_t *indices, const float *log_rest,
+                            const float *weights, float temperature, float scale, int mean, const float *factor,
+                            int holds, void *grad, void *workspace, size_t workspace_bytes, tropnn_stream_t stream) {
+    tropnn::LogitRows x{};
+    if (int rc = check_distill(rows, vocab, row_stride, logits, dtype, k, values, values_dtype, indices, log_rest, weights,
+                               temperature, grad, workspace, workspace_bytes, x))
+        return rc;
+    if (rows == 0) return abi_ok();
+    if (!factor || !grad) return abi_fail(TROPNN_ERR_INVALID_ARGUMENT, "factor and grad must be non-NULL");
+    if (misaligned(factor, 4)) return abi_fail(TROPNN_ERR_INVALID_ARGUMENT, "factor must be aligned to its elements");
+    const tropnn::DistillArgs a{x, values, indices, log_rest, weights, static_cast<int>(k), values_dtype, mean != 0,
+                                temperature, scale, nullptr, grad, factor, holds != 0};
+    return launched("distillation gradient launch", tropnn::launch_distill(a, workspace, static_cast<hipStream_t>(stream)));
 }
 
 int tropnn_hip_scale_in_place(int64_t n, void *x, int dtype, const float *factor, tropnn_stream_t stream) {

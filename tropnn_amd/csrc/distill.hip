@@ -27,7 +27,12 @@ struct DistillKernelArgs {
     float temperature, scale;
     float *row_loss;
     void *grad;
+    const float *factor;  // of the gradient, or NULL: 1
+    bool holds;           // grad has the gradient for a factor of one
     int bitmap_words;
+
+    // Nothing is left to do where a gradient that is there is multiplied by one.
+    __device__ __forceinline__ bool done(float f) const { return holds && f == 1.f; }
 };
 
 __device__ __forceinline__ float any_value(const void *p, int dtype, int64_t i) {
@@ -201,7 +206,8 @@ struct RowWork {
 
     // From the workgroup's sum s around `reference` and the list's sums.
     __device__ __forceinline__ RowTotals totals(int64_t row, float s, float reference, const ListSums &list, float x_tail,
-                                                const uint32_t *bits, float *scratch, float weight, float norm, int tid) const {
+                                                const uint32_t *bits, float *scratch, float weight, float norm, float factor,
+                                                int tid) const {
         ExpSum teacher = exp_sum(list.teacher_m, list.teacher_s);
         const float r = rest(row);
         if (REST) teacher.join(ExpSum::of(r), c);
@@ -240,7 +246,7 @@ struct RowWork {
         t.l_teacher = log2f(teacher.s);
         t.log_p0 = t.log_p(r, c);
         t.log_q0 = t.none ? -INFINITY : fmaf(t.ref - all.m, c, t.l_ref - t.l);
-        t.scale = a.temperature * a.scale * weight / norm;
+        t.scale = a.temperature * a.scale * weight / norm * factor;
         return t;
     }
 
@@ -351,6 +357,8 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillKernelArgs
     __shared__ float sums[2][2 * kWaves], parts[kWaves];
     __shared__ ListSums lists[kWaves];
     const W k(args);
+    const float factor = args.factor ? *args.factor : 1.f;
+    if (args.done(factor)) return;
     const int words = REST ? args.bitmap_words : 0;
     const float norm = args.norm ? *args.norm : args.norm_value;
     const int64_t rows = args.rows, grid = gridDim.x;
@@ -406,7 +414,7 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillKernelArgs
         s += fast_exp2(fmaf(k.unlisted_tail(x_tail, bits, tid), k.c, -offset));
         s = block_total<THREADS>(s, sums[0], tid);
         const bool dead = __builtin_amdgcn_readfirstlane(list.entries == 0.f);  // nothing to learn from this row
-        const RowTotals t = k.totals(row, dead ? 1.f : s, reference, list, x_tail, bits, sums[1], weight, norm, tid);
+        const RowTotals t = k.totals(row, dead ? 1.f : s, reference, list, x_tail, bits, sums[1], weight, norm, factor, tid);
         if (tid / kWave < k.list_waves()) {
             const float part = k.loss_part(row, first, t, tid);
             if ((tid & (kWave - 1)) == 0) parts[tid / kWave] = dead ? 0.f : part;
@@ -461,6 +469,8 @@ __global__ __launch_bounds__(THREADS) void distill_stream_kernel(DistillKernelAr
     __shared__ float sums[2][2 * kWaves], parts[kWaves];
     __shared__ ListSums lists[kWaves];
     const W k(args);
+    const float factor = GRAD && args.factor ? *args.factor : 1.f;
+    if (args.done(factor)) return;
     const int tid = threadIdx.x;
     const int64_t row = args.first_row + blockIdx.x;
     const float norm = args.norm ? *args.norm : args.norm_value, weight = k.weight(row);
@@ -499,7 +509,7 @@ __global__ __launch_bounds__(THREADS) void distill_stream_kernel(DistillKernelAr
         if (tid == 0) args.row_loss[row] = 0.f;
         return;
     }
-    const RowTotals t = k.totals(row, s, reference, list, x_tail, listed_bits, sums[1], weight, norm, tid);
+    const RowTotals t = k.totals(row, s, reference, list, x_tail, listed_bits, sums[1], weight, norm, factor, tid);
     if (tid / kWave < k.list_waves()) {
         const float part = k.loss_part(row, first, t, tid);
         if ((tid & (kWave - 1)) == 0) parts[tid / kWave] = part;
@@ -635,8 +645,8 @@ hipError_t launch_distill(const DistillArgs &a, void *workspace, hipStream_t str
     const bool sum_weights = a.mean && a.weights;
     DistillKernelArgs k{a.x.p, a.x.rows, a.x.stride, 0, a.x.vocab, a.k, a.values_dtype, a.values, a.indices, a.log_rest, a.weights,
                         sum_weights ? norm : nullptr, a.mean ? static_cast<float>(a.x.rows) : 1.f, a.temperature,
-                        a.scale, row_loss, a.grad, 0};
-    if (sum_weights) {
+                        a.scale, row_loss, a.grad, a.factor, a.holds, 0};
+    if (sum_weights && !a.holds) {
         hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kSumThreads), 0, stream, a.weights, a.x.rows, 1.f,
                            static_cast<const float *>(nullptr), 1.f, norm);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -646,6 +656,7 @@ hipError_t launch_distill(const DistillArgs &a, void *workspace, hipStream_t str
         hipError_t e = with_logit_type(a.x.dtype, [&](auto t) { return launch_by_width<decltype(t)>(k, stream); });
         if (e != hipSuccess) return e;
     }
+    if (!a.loss) return hipSuccess;
     hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kSumThreads), 0, stream, static_cast<const float *>(row_loss),
                        a.x.rows, a.scale, static_cast<const float *>(k.norm), k.norm_value, a.loss);
     return hipGetLastError();

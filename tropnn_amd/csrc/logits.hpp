@@ -32,8 +32,10 @@ struct DistillArgs {
     const float *log_rest, *weights;
     int k, values_dtype, mean;
     float temperature, scale;
-    float *loss;
+    float *loss;  // NULL: the gradient alone
     void *grad;
+    const float *factor;  // of the gradient, or NULL: 1
+    bool holds;           // grad and the workspace are as a call without a factor left them
 };
 size_t distill_workspace(const LogitRows &x, int k, bool want_grad);
 hipError_t launch_distill(const DistillArgs &a, void *workspace, hipStream_t stream);

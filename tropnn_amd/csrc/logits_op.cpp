@@ -5,11 +5,15 @@
 // only: every launch goes through the C ABI of libtropnn_hip.so
 // (include/tropnn_hip_logits.h), whose addresses the Python package hands over.
 //
-// The forward's launch writes the gradient too. The backward hands it over,
-// scaled in place by the incoming gradient (a kernel reads that, and leaves the
-// gradient alone where it is one), and gives it up, so that autograd can keep
-// it as the logits' grad without a copy. A second backward through the same
-// node computes it again from the saved inputs.
+// The forward's launch writes the gradient too. The backward hands it over and
+// gives it up, so that autograd can keep it as the logits' grad without a copy.
+// An incoming gradient that the host does not know to be one is read by a
+// kernel, which leaves the gradient alone where it is one after all. Otherwise
+// an f32 gradient is scaled in place, and a 16-bit one is computed again with
+// the factor before its rounding: a loss scaled against f16's underflow needs
+// the bits that the unscaled gradient does not have. Either moves as many bytes
+// (a read and a write of the gradient's size). A second backward through the
+// same node computes the gradient again from the saved inputs.
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
@@ -34,21 +38,23 @@ using torch::autograd::variable_list;
 struct LogitsAbi {
     decltype(&tropnn_hip_distill) distill = nullptr;
     decltype(&tropnn_hip_distill_workspace_size) distill_workspace_size = nullptr;
+    decltype(&tropnn_hip_distill_grad) distill_grad = nullptr;
     decltype(&tropnn_hip_scale_in_place) scale_in_place = nullptr;
     decltype(&tropnn_hip_last_error) last_error = nullptr;
 };
 LogitsAbi g_logits_abi;
 std::atomic<bool> g_logits_bound{false};
 
-void bind_logits_abi(int64_t distill, int64_t distill_workspace_size, int64_t scale_in_place, int64_t last_error,
-                     int64_t abi_version) {
+void bind_logits_abi(int64_t distill, int64_t distill_workspace_size, int64_t distill_grad, int64_t scale_in_place,
+                     int64_t last_error, int64_t abi_version) {
     TORCH_CHECK(abi_version == TROPNN_HIP_LOGITS_ABI_VERSION, "libtropnn_hip.so has logits ABI version ", abi_version,
                 ", the autograd operator was built for ", TROPNN_HIP_LOGITS_ABI_VERSION);
-    TORCH_CHECK(distill != 0 && distill_workspace_size != 0 && scale_in_place != 0 && last_error != 0,
+    TORCH_CHECK(distill != 0 && distill_workspace_size != 0 && distill_grad != 0 && scale_in_place != 0 && last_error != 0,
                 "bind_logits_abi: NULL entry point");
     auto set = [](auto &f, int64_t address) { f = reinterpret_cast<std::decay_t<decltype(f)>>(static_cast<intptr_t>(address)); };
     set(g_logits_abi.distill, distill);
     set(g_logits_abi.distill_workspace_size, distill_workspace_size);
+    set(g_logits_abi.distill_grad, distill_grad);
     set(g_logits_abi.scale_in_place, scale_in_place);
     set(g_logits_abi.last_error, last_error);
     g_logits_bound.store(true, std::memory_order_release);
@@ -95,34 +101,49 @@ Rows as_rows(const Tensor &logits) {
     return {logits.contiguous(), rows, vocab, vocab};
 }
 
-struct Loss {
-    Tensor loss, grad;
+// An operator's inputs as the entry points take them.
+struct Inputs {
+    Rows x;
+    Tensor values, indices, log_rest, weights;
+    int64_t k;
+    int dtype, values_dtype;
+    double temperature, scale;
+    bool mean;
+
+    Inputs(const Tensor &logits, const Tensor &v, const Tensor &at, const std::optional<Tensor> &rest,
+           const std::optional<Tensor> &w, double t, double s, bool m)
+        : x(as_rows(logits)), values(v.contiguous()), indices(at.contiguous()),
+          log_rest(rest.has_value() ? rest->contiguous() : Tensor()), weights(w.has_value() ? w->contiguous() : Tensor()),
+          k(v.size(-1)), dtype(logit_type(logits)), values_dtype(logit_type(v)), temperature(t), scale(s), mean(m) {
+        TORCH_CHECK(g_logits_bound.load(std::memory_order_acquire), "tropnn_hip.distill: the C ABI is not bound");
+    }
+    Tensor workspace() const {
+        const size_t bytes = g_logits_abi.distill_workspace_size(x.rows, x.vocab, dtype, k, 1);
+        return at::empty({static_cast<int64_t>(bytes)}, x.t.options().dtype(at::kByte));
+    }
+    // Calls `entry` with the inputs, `out...`, the workspace and the stream.
+    template <typename F, typename... Out>
+    void call(const char *what, F entry, const Tensor &ws, Out... out) const {
+        check(entry(x.rows, x.vocab, x.stride, x.t.const_data_ptr(), dtype, k, values.const_data_ptr(), values_dtype,
+                    indices.const_data_ptr<int64_t>(), log_rest.defined() ? log_rest.const_data_ptr<float>() : nullptr,
+                    weights.defined() ? weights.const_data_ptr<float>() : nullptr, static_cast<float>(temperature),
+                    static_cast<float>(scale), mean, out..., ws.mutable_data_ptr(), ws.nbytes(),
+                    c10::hip::getCurrentHIPStream(x.t.device().index()).stream()),
+              what);
+    }
 };
 
-Loss run_distill(const Tensor &logits, const Tensor &values, const Tensor &indices, const std::optional<Tensor> &log_rest,
-                 const std::optional<Tensor> &weights, double temperature, double scale, bool mean, bool want_grad) {
-    TORCH_CHECK(g_logits_bound.load(std::memory_order_acquire), "tropnn_hip.distill: the C ABI is not bound");
-    const c10::DeviceGuard guard(logits.device());
-    const Rows x = as_rows(logits);
-    const Tensor v = values.contiguous(), at = indices.contiguous();
-    const Tensor rest = log_rest.has_value() ? log_rest->contiguous() : Tensor();
-    const Tensor w = weights.has_value() ? weights->contiguous() : Tensor();
-    const auto f32 = logits.options().dtype(at::kFloat);
+struct Loss {
+    Tensor loss, grad, workspace;
+};
+
+Loss run_distill(const Tensor &logits, const Inputs &in, bool want_grad) {
     Loss out;
-    out.loss = at::empty({}, f32);
+    out.loss = at::empty({}, logits.options().dtype(at::kFloat));
     if (want_grad) out.grad = at::empty(logits.sizes(), logits.options());
-    const int dtype = logit_type(logits);
-    const int64_t k = values.size(-1);
-    const size_t bytes = g_logits_abi.distill_workspace_size(x.rows, x.vocab, dtype, k, want_grad);
-    const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, f32.dtype(at::kByte));
-    check(g_logits_abi.distill(x.rows, x.vocab, x.stride, x.t.const_data_ptr(), dtype, k, v.const_data_ptr(),
-                               logit_type(v), at.const_data_ptr<int64_t>(),
-                               rest.defined() ? rest.const_data_ptr<float>() : nullptr,
-                               w.defined() ? w.const_data_ptr<float>() : nullptr, static_cast<float>(temperature),
-                               static_cast<float>(scale), mean, out.loss.mutable_data_ptr<float>(),
-                               want_grad ? out.grad.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), bytes,
-                               c10::hip::getCurrentHIPStream(logits.device().index()).stream()),
-          "tropnn_hip_distill");
+    out.workspace = in.workspace();
+    in.call("tropnn_hip_distill", g_logits_abi.distill, out.workspace, out.loss.mutable_data_ptr<float>(),
+            want_grad ? out.grad.mutable_data_ptr() : nullptr);
     return out;
 }
 
@@ -133,14 +154,27 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
     static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &values, const Tensor &indices,
                           const std::optional<Tensor> &log_rest, const std::optional<Tensor> &weights, double temperature,
                           double scale, bool mean, const std::optional<Tensor> &unit) {
-        Loss out = run_distill(logits, values, indices, log_rest, weights, temperature, scale, mean, true);
+        const c10::DeviceGuard guard(logits.device());
+        const Inputs in(logits, values, indices, log_rest, weights, temperature, scale, mean);
+        Loss out = run_distill(logits, in, true);
         ctx->save_for_backward({logits, values, indices, log_rest.value_or(Tensor()), weights.value_or(Tensor())});
         ctx->saved_data["grad"] = std::move(out.grad);
+        if (in.dtype != TROPNN_LOGITS_F32) ctx->saved_data["workspace"] = std::move(out.workspace);
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["mean"] = mean;
         if (unit.has_value()) ctx->saved_data["unit"] = *unit;
         return out.loss;
+    }
+
+    // A tensor of the context's own, which it then no longer has; undefined
+    // where it has none.
+    static Tensor take(AutogradContext *ctx, const char *name) {
+        const auto it = ctx->saved_data.find(name);
+        if (it == ctx->saved_data.end()) return Tensor();
+        Tensor t = it->second.toTensor();
+        ctx->saved_data.erase(it);
+        return t;
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grad_outputs) {
@@ -150,27 +184,31 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0];
         const c10::DeviceGuard guard(logits.device());
-        Tensor grad;
-        if (auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {
-            grad = it->second.toTensor();
-            ctx->saved_data.erase(it);
-        } else {
-            grad = run_distill(logits, saved[1], saved[2], some(saved[3]), some(saved[4]),
-                               ctx->saved_data["temperature"].toDouble(), ctx->saved_data["scale"].toDouble(),
-                               ctx->saved_data["mean"].toBool(), true)
-                       .grad;
-        }
         bool one = false;  // known on the host
         if (auto it = ctx->saved_data.find("unit"); it != ctx->saved_data.end()) {
             const Tensor unit = it->second.toTensor();
             one = unit._version() == 0 && unit.const_data_ptr() == incoming.const_data_ptr();
         }
-        if (!one) {
+        Tensor grad = take(ctx, "grad"), workspace = take(ctx, "workspace");
+        if (!(grad.defined() && one)) {
             const Tensor factor = incoming.to(at::kFloat).contiguous();
-            check(g_logits_abi.scale_in_place(grad.numel(), grad.mutable_data_ptr(), logit_type(grad),
-                                              factor.const_data_ptr<float>(),
-                                              c10::hip::getCurrentHIPStream(grad.device().index()).stream()),
-                  "tropnn_hip_scale_in_place");
+            const float *f = factor.const_data_ptr<float>();
+            if (grad.defined() && logit_type(grad) == TROPNN_LOGITS_F32) {
+                check(g_logits_abi.scale_in_place(grad.numel(), grad.mutable_data_ptr(), TROPNN_LOGITS_F32, f,
+                                                  c10::hip::getCurrentHIPStream(grad.device().index()).stream()),
+                      "tropnn_hip_scale_in_place");
+            } else {
+                const Inputs in(logits, saved[1], saved[2], some(saved[3]), some(saved[4]),
+                                ctx->saved_data["temperature"].toDouble(), ctx->saved_data["scale"].toDouble(),
+                                ctx->saved_data["mean"].toBool());
+                const bool holds = grad.defined();
+                if (!holds) {
+                    grad = at::empty(logits.sizes(), logits.options());
+                    workspace = in.workspace();
+                }
+                in.call("tropnn_hip_distill_grad", g_logits_abi.distill_grad, workspace, f, static_cast<int>(holds),
+                        grad.mutable_data_ptr());
+            }
         }
         grads[0] = std::move(grad);
         return grads;
@@ -182,14 +220,15 @@ Tensor distill(const Tensor &logits, const Tensor &values, const Tensor &indices
                const std::optional<Tensor> &unit) {
     if (at::GradMode::is_enabled() && logits.requires_grad())
         return DistillFunction::apply(logits, values, indices, log_rest, weights, temperature, scale, mean, unit);
-    return run_distill(logits, values, indices, log_rest, weights, temperature, scale, mean, false).loss;
+    const c10::DeviceGuard guard(logits.device());
+    return run_distill(logits, Inputs(logits, values, indices, log_rest, weights, temperature, scale, mean), false).loss;
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(tropnn_hip, m) {
-    m.def("bind_logits_abi(int distill, int distill_workspace_size, int scale_in_place, int last_error, "
-          "int abi_version) -> ()",
+    m.def("bind_logits_abi(int distill, int distill_workspace_size, int distill_grad, int scale_in_place, "
+          "int last_error, int abi_version) -> ()",
           &bind_logits_abi);
     // the layout that distill reads logits in, for any device: (tensor, rows, vocab, row stride)
     m.def("logit_rows(Tensor logits) -> (Tensor, int, int, int)", [](const Tensor &logits) {

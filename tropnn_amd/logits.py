@@ -120,8 +120,10 @@ def distillation_loss(
     over the rows, which also reads them only once from memory where they fit
     the caches; without a gradient asked for, the loss alone is computed. The
     backward pass from a gradient of one (loss.backward(), or a sum of losses'
-    backward) leaves it at that; another value costs a pass over the gradient,
-    which `scale` spares."""
+    backward) leaves it at that; another value costs a pass over the gradient
+    (16-bit ones are computed again, with that value before their rounding, so
+    that a loss scaled against underflow keeps its small gradients), which
+    `scale` spares."""
     name = "distillation_loss"
     _check_logits(name, logits)
     lead = logits.shape[:-1]
