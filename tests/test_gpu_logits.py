@@ -800,3 +800,32 @@ def test_distillation_scaled_loss_in_a_graph():
         want = run()
         _ = torch.ones(64, device=DEV).sum().item()
         assert torch.equal(out, want), rep
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_distillation_has_no_second_derivative(dtype):
+    """With create_graph the gradient is the same, and whatever would need its
+    derivative raises instead of leaving that part out."""
+    values, indices, log_rest = make_record(4, 257, 6, 2)
+    x = rows_of(4, 257, dtype, 1).requires_grad_(True)
+    (want,) = torch.autograd.grad(distillation_loss(x, values, indices, log_rest), x)
+
+    def loss_and_grad(**kw):
+        loss = distillation_loss(x, values, indices, log_rest)
+        return loss, torch.autograd.grad(loss, x, create_graph=True, **kw)[0]
+
+    loss, grad = loss_and_grad()
+    assert torch.equal(grad, want) and grad.requires_grad
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        (loss + grad.float().square().sum()).backward()
+    _, grad = loss_and_grad()
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(grad.float().square().sum(), x, allow_unused=True)
+    incoming = torch.tensor(2.0, device=DEV, requires_grad=True)  # nor the derivative by the incoming gradient
+    _, grad = loss_and_grad(grad_outputs=incoming)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(grad.float().sum(), incoming)
+    # a graph that does not go through it
+    distillation_loss(x, values, indices, log_rest).backward(create_graph=True)
+    assert torch.equal(x.grad.detach(), want)
+    x.grad = None

@@ -13,13 +13,17 @@
 // the factor before its rounding: a loss scaled against f16's underflow needs
 // the bits that the unscaled gradient does not have. Either moves as many bytes
 // (a read and a write of the gradient's size). A second backward through the
-// same node computes the gradient again from the saved inputs.
+// same node computes the gradient again from the saved inputs. The gradient has
+// no derivative of its own: where a graph of the backward is made, it hangs on a
+// node that raises.
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <atomic>
@@ -181,6 +185,8 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         variable_list grads(9);  // one per forward argument
         const Tensor &incoming = grad_outputs[0];
         if (!incoming.defined()) return grads;
+        const bool graph = at::GradMode::is_enabled();  // of this backward (create_graph)
+        const at::NoGradGuard no_grad;
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0];
         const c10::DeviceGuard guard(logits.device());
@@ -210,6 +216,12 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
                         grad.mutable_data_ptr());
             }
         }
+        if (graph)
+            torch::autograd::set_history(
+                grad, std::make_shared<torch::autograd::Error>(
+                          "distillation_loss: a derivative of its gradient was asked for, which it does not have "
+                          "(the operator can be differentiated once)",
+                          torch::autograd::collect_next_edges(logits, incoming)));
         grads[0] = std::move(grad);
         return grads;
     }
