@@ -829,3 +829,23 @@ def test_distillation_has_no_second_derivative(dtype):
     distillation_loss(x, values, indices, log_rest).backward(create_graph=True)
     assert torch.equal(x.grad.detach(), want)
     x.grad = None
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_distillation_has_no_forward_mode_derivative(requires_grad):
+    """A dual number is refused, where its tangent would be dropped; outside of
+    the level the same logits are taken."""
+    import torch.autograd.forward_ad as forward_ad
+
+    values, indices, log_rest = make_record(4, 257, 6, 2)
+    x = rows_of(4, 257, F32, 1).requires_grad_(requires_grad)
+    want = distillation_loss(x, values, indices, log_rest).detach()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            distillation_loss(dual, values, indices, log_rest)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            distillation_loss(dual, values, indices, log_rest)
+        assert torch.equal(distillation_loss(x, values, indices, log_rest).detach(), want)
+        assert torch.equal(distillation_loss(dual.detach(), values, indices, log_rest), want)
+    assert torch.equal(distillation_loss(x, values, indices, log_rest).detach(), want)

@@ -230,6 +230,8 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
 Tensor distill(const Tensor &logits, const Tensor &values, const Tensor &indices, const std::optional<Tensor> &log_rest,
                const std::optional<Tensor> &weights, double temperature, double scale, bool mean,
                const std::optional<Tensor> &unit) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!logits._fw_grad(/*level=*/0).defined(),
+                                "distillation_loss: forward-mode differentiation is not supported");
     if (at::GradMode::is_enabled() && logits.requires_grad())
         return DistillFunction::apply(logits, values, indices, log_rest, weights, temperature, scale, mean, unit);
     const c10::DeviceGuard guard(logits.device());

@@ -117,7 +117,8 @@ def distillation_loss(
     where that is 0), or "sum". scale multiplies the result.
 
     Gradients flow to the logits alone, once: a derivative of the gradient
-    (create_graph) raises RuntimeError where it is asked for. Loss and gradient come from one launch
+    (create_graph) raises RuntimeError where it is asked for, a forward-mode
+    derivative NotImplementedError. Loss and gradient come from one launch
     over the rows, which also reads them only once from memory where they fit
     the caches; without a gradient asked for, the loss alone is computed. The
     backward pass from a gradient of one (loss.backward(), or a sum of losses'
