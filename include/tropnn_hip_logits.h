@@ -45,7 +45,7 @@ int tropnn_hip_logits_abi_version(void);
  *   indices [rows][k]  int64
  *   log_rest [rows]    f32, log sum over the other logits x of
  *                      exp(x / temperature); -inf where there are none, or
- *                      all of them are -inf
+ *                      all of them are -inf; NaN where one is
  */
 size_t tropnn_hip_top_logits_workspace_size(int64_t rows, int64_t vocab, int dtype, int64_t k);
 int tropnn_hip_top_logits(int64_t rows, int64_t vocab, int64_t row_stride, const void *logits, int dtype, int64_t k,

@@ -849,3 +849,18 @@ def test_distillation_has_no_forward_mode_derivative(requires_grad):
         assert torch.equal(distillation_loss(x, values, indices, log_rest).detach(), want)
         assert torch.equal(distillation_loss(dual.detach(), values, indices, log_rest), want)
     assert torch.equal(distillation_loss(x, values, indices, log_rest).detach(), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [60, 1000, 33000, 100003])
+def test_top_logits_nan_and_infinity_among_the_others(vocab, dtype):
+    """More NaNs than the list holds beside infinities of either sign: the
+    log-mass of the others is NaN; infinities alone make it infinite."""
+    x = rows_of(6, vocab, dtype, 3)
+    for r, (nans, inf) in enumerate(((15, math.inf), (15, -math.inf), (5, math.inf), (4, math.inf), (0, math.inf), (15, 0.0))):
+        x[r, vocab // 3 : vocab // 3 + nans] = math.nan
+        x[r, [1, vocab - 2]] = inf
+    x[5, :] = torch.where(torch.isnan(x[5]), x[5], -math.inf)
+    for k in (1, 4, 14):
+        check_top(x, k)
+        check_top(x, k, temperature=0.3)

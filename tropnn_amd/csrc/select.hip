@@ -798,7 +798,8 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(TopKernelArgs a)
             o.s = sh.wave_rest[w].y;
             rest.join(o, c);
         }
-        a.log_rest[r] = rest.m == INFINITY ? INFINITY : rest.m / a.temperature + logf(rest.s);
+        // infinite logits, but not beside a NaN
+        a.log_rest[r] = rest.m == INFINITY && rest.s == rest.s ? INFINITY : rest.m / a.temperature + logf(rest.s);
     }
 }
 
