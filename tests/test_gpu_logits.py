@@ -864,3 +864,30 @@ def test_top_logits_nan_and_infinity_among_the_others(vocab, dtype):
     for k in (1, 4, 14):
         check_top(x, k)
         check_top(x, k, temperature=0.3)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_distillation_gradient_is_rounded_once_far_from_zero(dtype):
+    """The teacher's list lies 2^80 below the student's other logits, around
+    2^190: the constants of the gradient's exponents are at their largest.
+    In f32, an exponent off by e moves a gradient by e ln 2 of itself. A constant
+    below 2^8 is off by 2^-17 at most, a log-sum below 2^7 by 2^-18, half an ulp
+    each, the instruction and the row's factor by 4 u: 1e-5 of a gradient, beside
+    the half ulp of the type's own rounding. A constant above 2^8 would be off by
+    2^-16."""
+    rows, vocab, k = 20000, 64, 3
+    gen = torch.Generator().manual_seed(7)
+    x = 180.0 + 6.0 * torch.rand(rows, vocab, generator=gen)
+    indices = torch.rand(rows, vocab, generator=gen).argsort(1)[:, :k].contiguous()
+    x.scatter_(1, indices, 131.0 - 3.0 * torch.rand(rows, k, generator=gen))
+    logits = x.to(dtype).to(DEV).requires_grad_(True)
+    values = torch.zeros(rows, k, device=DEV)
+    distillation_loss(logits, values, indices.to(DEV), reduction="sum").backward()
+    want = torch.softmax(logits.detach().double(), 1)  # of a class outside the list
+    near_zero = 2.0**-13  # above f16's subnormal numbers
+    mantissa, exponent = torch.frexp(want)
+    half_ulp = torch.ldexp(torch.ones_like(mantissa), exponent - (12 if dtype == F16 else 9))
+    off = ((logits.grad.double() - want).abs() - half_ulp) / want
+    off.scatter_(1, indices.to(DEV), 0.0)
+    assert (want > near_zero).double().mean() > 0.5
+    assert off[want > near_zero].max() <= 1e-5

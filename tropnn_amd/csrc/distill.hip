@@ -269,9 +269,9 @@ struct RowWork {
     }
 
     // Gradients of classes outside the list. `near`: the difference and the
-    // product with c as one multiply-add from a constant below 2^8, whose
-    // rounding to 2^-16 moves a gradient by 2^-17 of itself, far below the
-    // rounding to 16 bits.
+    // product with c as one multiply-add from `from`. Below 2^8 it is a multiple
+    // of 2^-16, so its rounding moves a gradient by 2^-17 of itself at most, far
+    // below the rounding to 16 bits.
     struct Outer {
         float by, from, ref, l_ref, c;
         bool near;
@@ -285,8 +285,8 @@ struct RowWork {
         o.ref = t.ref;
         o.l_ref = t.l_ref;
         o.c = c;
-        o.near = sizeof(T) == 2 && __builtin_amdgcn_readfirstlane(fabsf(t.ref * c) < 200.f);
         o.from = fmaf(-t.ref, c, -t.l_ref);
+        o.near = sizeof(T) == 2 && __builtin_amdgcn_readfirstlane(fabsf(o.from) < 256.f);
         return o;
     }
     __device__ __forceinline__ void store(T *to, int first, int tid, const words4 &v) const {
