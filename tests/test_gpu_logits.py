@@ -891,3 +891,13 @@ def test_distillation_gradient_is_rounded_once_far_from_zero(dtype):
     off.scatter_(1, indices.to(DEV), 0.0)
     assert (want > near_zero).double().mean() > 0.5
     assert off[want > near_zero].max() <= 1e-5
+
+
+def test_sample_top_k_of_any_int64():
+    """0 and less are no limit, however far below; more than the classes is all."""
+    logits = rows_of(8, 700, F32, 2)
+    u = torch.full((8,), 0.97, device=DEV)
+    top_k = torch.tensor([0, -1, -(2**31) - 5, 5 - 2**32, -(2**63), 2**31 + 1, 2**63 - 1, 3], device=DEV)
+    got, want = sample_tokens(logits, u, top_k=top_k), sample_tokens(logits, u)
+    assert torch.equal(got.tokens[:7], want.tokens[:7]) and torch.equal(got.log_probs[:7], want.log_probs[:7])
+    assert int(got.tokens[7]) in order_of(logits[7].cpu())[1][:3].tolist()

@@ -191,7 +191,7 @@ def sample_tokens(
                 raise ValueError(f"{name} needs min_p in [0, 1], got {value}")
     if isinstance(top_k, Tensor):
         _check_other(name, "top_k", top_k, logits, lead, (torch.int32, torch.int64))
-        top_k = top_k.clamp(max=MAX_VOCAB).to(torch.int32) if top_k.dtype == torch.int64 else top_k
+        top_k = top_k.clamp(0, MAX_VOCAB).to(torch.int32) if top_k.dtype == torch.int64 else top_k
     else:
         top_k = min(max(int(top_k), 0), MAX_VOCAB)
     return SampledTokens(*sample_hip(logits.detach(), uniforms, floats["temperature"], top_k, floats["top_p"], floats["min_p"]))
