@@ -901,3 +901,68 @@ def test_sample_top_k_of_any_int64():
     got, want = sample_tokens(logits, u, top_k=top_k), sample_tokens(logits, u)
     assert torch.equal(got.tokens[:7], want.tokens[:7]) and torch.equal(got.log_probs[:7], want.log_probs[:7])
     assert int(got.tokens[7]) in order_of(logits[7].cpu())[1][:3].tolist()
+
+
+@pytest.mark.parametrize("rest,weighted", [(True, True), (False, True), (True, False)])
+@pytest.mark.parametrize(
+    "rows,vocab,k,dtype,grid",
+    [  # one more row than the workgroups, or several for each; the numbers of threads and of pieces a thread
+        (4099, 10, 4, F32, 4096),
+        (9001, 40, 9, F32, 4096),
+        (9001, 700, 130, F32, 4096),
+        (8500, 3101, 70, BF16, 4096),
+        (3300, 5003, 33, BF16, 1536),
+        (3300, 5003, 17, F32, 1536),
+        (1301, 20000, 64, F16, 512),
+        (1301, 20003, 5, F32, 512),
+        (700, 70003, 300, BF16, 256),
+    ],
+)
+def test_distillation_several_rows_a_workgroup(rows, vocab, k, dtype, grid, rest, weighted):
+    """More rows than workgroups that hold them (`grid`): every one has its next
+    row's list and pieces under way, rows of weight 0 and without a list in
+    between, first, last and alone."""
+    gen = torch.Generator().manual_seed(rows + k)
+    logits = rows_of(rows, vocab, dtype, rows, pad=1)
+    teacher = torch.randn(rows, vocab, generator=torch.Generator(device=DEV).manual_seed(k), device=DEV) * 3
+    values, indices = torch.sort(teacher, dim=1, descending=True, stable=True)
+    log_rest = torch.logsumexp(values[:, k:].double(), 1).float() if rest else None
+    values, indices = values[:, :k].to(dtype), indices[:, :k].clone()
+    length = torch.where(torch.rand(rows, generator=gen) < 0.5, k, torch.randint(1, k + 1, (rows,), generator=gen))
+    for empty in (slice(3, 5), slice(11, None, grid), slice(grid + 1, grid + 3), slice(rows - 2, rows - 1)):
+        length[empty] = 0
+    far = [r for r in (6, grid, grid + 6, 2 * grid + 6) if r < rows]  # their sums leave the unit of the list's largest
+    length[far] = k
+    for r in far:
+        listed = logits[r].gather(0, indices[r])
+        logits[r] += 200.0
+        logits[r].scatter_(0, indices[r], listed)
+    indices[torch.arange(k, device=DEV) >= length.to(DEV)[:, None]] = -1
+    weights = None
+    if weighted:
+        weights = torch.where(torch.rand(rows, generator=gen) < 0.3, 0.0, 0.5 + torch.rand(rows, generator=gen))
+        for out in (slice(0, 3), slice(7, None, grid), slice(grid, grid + 2), slice(rows - 1, rows)):
+            weights[out] = 0.0
+        weights[5] = 1.0
+        weights[far] = 1.0
+        weights = weights.to(DEV)
+    want_loss, want, bound = distill_reference_by_rows(logits, values, indices, log_rest, weights)
+
+    def run():
+        x = logits.detach().requires_grad_(True)
+        loss = distillation_loss(x, values, indices, log_rest, weights=weights)
+        loss.backward()
+        return loss.detach(), x.grad
+
+    loss, grad = run()
+    assert abs(float(loss) - float(want_loss)) <= 2 * REL * (1 + abs(float(want_loss)))
+    for part in torch.arange(rows).split(max(1, (1 << 23) // vocab)):
+        part = slice(int(part[0]), int(part[-1]) + 1)
+        off = (grad[part].double() - want[part]).abs() - (bound[part] + HALF_ULP[dtype] * want[part].abs() + SMALLEST[dtype])
+        assert (off <= 0).all(), (part, off.max(), torch.nonzero((off > 0).any(1))[:5])
+    nothing = length.to(DEV) == 0
+    if weighted:
+        nothing |= weights == 0
+    assert not grad[nothing].any()
+    again = run()
+    assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
