@@ -966,3 +966,70 @@ def test_distillation_several_rows_a_workgroup(rows, vocab, k, dtype, grid, rest
     assert not grad[nothing].any()
     again = run()
     assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
+
+
+MOST = 1 << 20  # classes: the limit
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,k,shift", [(2, 1024, 0), (3, 5, 1), (1, 300, 3)])
+def test_top_logits_of_the_most_classes(rows, k, shift, dtype):
+    check_top(rows_of(rows, MOST, dtype, k, shift=shift), k, temperature=1.3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rest", [True, False])
+@pytest.mark.parametrize("vocab,k", [(MOST, 64), (MOST, 1024), (MOST - 3, 7), (516097, 20), (516096, 20), (516000, 20), (515000, 20)])
+def test_distillation_of_the_most_classes(vocab, k, rest, dtype):
+    """The limit, and around the vocabulary whose bitmap takes 64 KB of LDS. A
+    thread's run of a sum is 256 pieces at most, 2e-5 as for the sizes above."""
+    logits = rows_of(3, vocab, dtype, k)
+    values, indices, log_rest = make_record(3, vocab, k, 3, rest=rest, values_dtype=dtype)
+    indices[1, k // 2 :] = -1
+    indices[0, 0] = vocab - 1 if not (indices[0] == vocab - 1).any() else indices[0, 0]
+    check_distill(logits, values, indices, log_rest, torch.tensor([1.0, 2.0, 0.5], device=DEV))
+
+
+def sample_reference_wide(x, u, top_k=0, top_p=1.0, min_p=0.0):
+    """sample_reference for wide rows: whole logits [rows, vocab] (int64; hidden
+    ones far below), in whole numbers."""
+    m = x.amax(1, keepdim=True)
+    w = torch.where(m - x < 63, ONE >> (m - x).clamp(max=62), 0)
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices
+    kept = w.gather(1, order)
+    if top_k > 0:
+        kept[:, top_k:] = 0
+    before = kept.cumsum(1) - kept
+    if top_p < 1.0:
+        total = kept.sum(1, keepdim=True).double()
+        limit = (float(torch.tensor(top_p, dtype=F32)) * total).to(torch.int64).clamp(min=1)
+        kept = torch.where(before < limit, kept, 0)
+    kept = torch.where(kept.double() >= float(torch.tensor(min_p, dtype=F32)) * ONE, kept, 0)
+    by_index = torch.zeros_like(w).scatter(1, order, kept)
+    running = by_index.cumsum(1)
+    total = running[:, -1:]
+    target = torch.minimum((u.double()[:, None] * total.double()).to(torch.int64), total - 1)
+    token = (running <= target).sum(1, keepdim=True)
+    return token[:, 0], (by_index.gather(1, token).double() / total.double()).log()[:, 0]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [-6, -30])
+def test_sample_of_the_most_classes(low, dtype):
+    gen = torch.Generator().manual_seed(-low)
+    rows = 3
+    x = torch.randint(low, 1, (rows, MOST), generator=gen)
+    x[2] = -(torch.arange(MOST) % 97) - 1
+    x[2, MOST - 1] = 0  # the last class alone is the largest
+    x[:, 5:100] = -(1 << 20)  # masked
+    logits = torch.where(x < -1000, -math.inf, x.float()).to(dtype).to(DEV)
+    for n, kw in enumerate((dict(), dict(top_k=50), dict(top_k=1000, top_p=0.9), dict(top_k=5000), dict(top_p=0.9),
+                            dict(top_p=0.3, min_p=0.01), dict(min_p=0.2), dict(top_k=300000, top_p=0.5))):
+        u = torch.rand(rows, generator=gen)
+        u[0] = (0.0, 1.0 - 2.0**-24, 0.5)[n % 3]
+        got = sample_tokens(logits, u.to(DEV), temperature=LOG2E, **kw)
+        token, log_prob = sample_reference_wide(x, u, **kw)
+        assert torch.equal(got.tokens.cpu(), token), kw
+        assert torch.allclose(got.log_probs.cpu().double(), log_prob, rtol=1e-6, atol=1e-6), kw
+    cold = sample_tokens(logits, torch.zeros(rows, device=DEV), temperature=0.0)
+    assert torch.equal(cold.tokens.cpu(), torch.sort(x, dim=1, descending=True, stable=True).indices[:, 0])
