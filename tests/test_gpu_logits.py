@@ -1033,3 +1033,44 @@ def test_sample_of_the_most_classes(low, dtype):
         assert torch.allclose(got.log_probs.cpu().double(), log_prob, rtol=1e-6, atol=1e-6), kw
     cold = sample_tokens(logits, torch.zeros(rows, device=DEV), temperature=0.0)
     assert torch.equal(cold.tokens.cpu(), torch.sort(x, dim=1, descending=True, stable=True).indices[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [77, 3001, 50001])
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_p=0.5), dict(top_p=0.7, min_p=0.001), dict(min_p=0.05),
+                                dict(top_k=200, top_p=0.8), dict(top_k=25, top_p=0.95, min_p=0.01)])
+def test_sample_against_64_bits_with_wide_gaps(vocab, dtype, kw):
+    """As test_sample_against_64_bits, of rows whose cuts lie in wide gaps: 30
+    raised classes hold nearly all of the mass, a hundredth of it and more each,
+    and the others weigh a millionth of the largest, so that the cut is among the
+    raised ones and hardly ever within 1e-4 of the limit."""
+    rows, t = 200, 0.8
+    gen = torch.Generator().manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=gen) * 0.5 - 12.0
+    raised = torch.rand(rows, vocab, generator=gen).argsort(1)[:, :30]
+    x.scatter_(1, raised, torch.rand(rows, 30, generator=gen))
+    logits = x.to(dtype).to(DEV)
+    u = torch.rand(rows, generator=gen)
+    got = sample_tokens(logits, u.to(DEV), temperature=t, **kw)
+    values, order = order_of(logits.cpu())
+    w = torch.exp((values - values[:, :1]) / t)
+    top_k, top_p, min_p = kw.get("top_k", 0), kw.get("top_p", 1.0), kw.get("min_p", 0.0)
+    if top_k > 0:
+        w[:, top_k:] = 0.0
+    before = w.cumsum(1) - w
+    limit = top_p * w.sum(1, keepdim=True)
+    near = ((before - limit).abs() < 1e-4 * limit).any(1) & (top_p < 1)
+    near |= ((w - min_p).abs() < 1e-5).any(1) & (min_p > 0)
+    kept = w >= min_p
+    if top_p < 1:
+        kept &= before < limit
+    w = torch.where(kept, w, 0.0)
+    by_index = torch.zeros_like(w).scatter(1, order, w)
+    by_index /= by_index.sum(1, keepdim=True)
+    upto = by_index.cumsum(1)
+    token = got.tokens.cpu()[:, None]
+    p, high, ok = by_index.gather(1, token)[:, 0], upto.gather(1, token)[:, 0], ~near
+    assert ok.sum() >= 0.95 * rows
+    assert (p[ok] > 0).all()
+    assert ((u.double() <= high + 3e-5) & (u.double() >= high - p - 3e-5))[ok].all()
+    assert torch.allclose(got.log_probs.cpu().double()[ok], p[ok].log(), rtol=REL, atol=REL)
