@@ -89,7 +89,8 @@ def generate(model: Callable[[Tensor], Tensor], contexts: Tensor, steps: int, *,
              **sampling) -> tuple[Tensor, Tensor]:
     """`steps` tokens after each context and their log-probabilities, [batch,
     steps] both. The random numbers come from `generator`, one per token;
-    `sampling` is sample_tokens' temperature, top_k, top_p and min_p."""
+    `sampling` is sample_tokens' temperature, top_k, top_p and min_p. A token of
+    -1 (logits with a NaN: no answer) is followed as if it were class 0."""
     batch, context = contexts.shape
     uniforms = torch.rand(steps, batch, generator=generator, device=contexts.device)
     tokens, log_probs = [], []
@@ -98,7 +99,7 @@ def generate(model: Callable[[Tensor], Tensor], contexts: Tensor, steps: int, *,
         drawn = sample_tokens(model(window), uniforms[step], **sampling)
         tokens.append(drawn.tokens)
         log_probs.append(drawn.log_probs)
-        window = torch.cat([window, drawn.tokens.unsqueeze(1)], 1)[:, -context:]
+        window = torch.cat([window, drawn.tokens.clamp(min=0).unsqueeze(1)], 1)[:, -context:]
     return torch.stack(tokens, 1), torch.stack(log_probs, 1)
 
 
