@@ -28,3 +28,20 @@ def test_a_row_without_an_answer_does_not_index_with_it(monkeypatch):
     for window in seen:
         assert int(window.min()) >= 0
     assert seen[1].tolist() == [[2, 0], [4, 5], [8, 0]]
+
+
+def test_an_epochs_loss_is_the_mean_over_its_contexts(monkeypatch):
+    """Whatever batches they come in: a last one that is shorter, or one alone."""
+
+    def step(model, optimizer, contexts, rec, *, temperature):
+        return contexts.double().sum(1).mean()
+
+    monkeypatch.setattr(distill, "distill_step", step)
+    monkeypatch.setattr(distill, "FusedAdam", lambda *a, **kw: None)
+    monkeypatch.setattr(distill, "record", lambda teacher, contexts, k, temperature: [contexts])
+    monkeypatch.setattr(distill, "TopLogits", lambda *t: t)
+    monkeypatch.setattr(distill, "generate", lambda *a, **kw: None)
+    for contexts, batch in ((10, 4), (3, 512), (8, 4)):
+        out = distill.run(vocab=50, contexts=contexts, batch=batch, epochs=1, device="cpu")
+        want = distill.make_contexts(contexts, 50).double().sum(1).mean()
+        assert abs(out["losses"][0] - float(want)) <= 1e-5 * float(want)

@@ -118,8 +118,9 @@ def run(*, vocab: int = 512, contexts: int = 8192, batch: int = 512, k: int = 32
         for at in range(0, contexts, batch):
             rows = slice(at, at + batch)
             part = TopLogits(*(t[rows] for t in rec))
-            total += distill_step(student, optimizer, seen[rows], part, temperature=temperature).detach()
-        losses.append(float(total) / (contexts // batch))
+            loss = distill_step(student, optimizer, seen[rows], part, temperature=temperature)
+            total += loss.detach() * len(seen[rows])
+        losses.append(float(total) / contexts)
     answers = {}
     for name, model in (("teacher", teacher), ("student", student)):
         gen = torch.Generator(device=device).manual_seed(seed)
