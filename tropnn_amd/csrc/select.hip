@@ -1206,6 +1206,8 @@ int top_threads(const LogitRows &x, int pieces, int k) {
 // 56 / 32, 1024 39 / 84 / 53; of 8 rows, 1024 classes 256 9.0 / 15.6 / 10.3, 512
 // 7.4 / 12.2 / 10.3, 1024 8.3 / 13.0 / 12.0; 32768 512 9.2 / 19.7 / 11.8, 1024
 // 9.4 / 20.8 / 12.9; 65536 512 12.8 / 31.1 / 14.0, 1024 11.7 / 27.3 / 14.7.
+// A top_k of each row's own is on the device and plans nothing: rows whose own
+// is above the threads taken (256 at least) go by search.
 int sample_threads(const LogitRows &x, int pieces, int top_k) {
     const int by_row = x.rows >= kManyRows ? (pieces <= 2048 || top_k > 0 ? 256 : 512) : pieces <= 4096 ? 512 : 1024;
     return max(by_row, threads_for_list(top_k));

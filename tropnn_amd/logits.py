@@ -168,6 +168,11 @@ def sample_tokens(
     uniform number times their mass. Each parameter is one value, or a tensor [...]
     with every row's own (f32; top_k int32 or int64).
 
+    top_k up to 1024 as one value, and up to 256 as a row's own in any batch,
+    draws from a short list; a larger one may search the row instead, which reads
+    it several times. Not differentiable: log_probs is a number, no function of
+    the logits to train through.
+
     Probabilities are whole multiples of 2^-40 of the row's largest, so all
     sums are exact: a row's answer depends on that row and its number alone, not
     on the batch around it or on how the work is split. A row with a NaN, or
