@@ -78,9 +78,10 @@ int tropnn_hip_distill(int64_t rows, int64_t vocab, int64_t row_stride, const vo
  * The chain rule's product of that gradient with the incoming one, factor[0]:
  * grad = factor[0] * d loss / d logits, rounded once to `dtype`. The arguments
  * are those of tropnn_hip_distill and `grad` is non-NULL; no loss is given.
- * holds != 0: grad is what tropnn_hip_distill wrote for the same arguments and
- * workspace that call's, neither touched since. Where factor[0] is 1, grad is
- * then left alone. holds == 0: the contents of both are irrelevant.
+ * holds != 0: grad is what tropnn_hip_distill wrote for the same arguments and,
+ * where the mean is weighted (mean != 0 and weights), workspace is that call's,
+ * neither touched since. Where factor[0] is 1, grad is then left alone.
+ * holds == 0: the contents of both are irrelevant.
  */
 int tropnn_hip_distill_grad(int64_t rows, int64_t vocab, int64_t row_stride, const void *logits, int dtype, int64_t k,
                             const void *values, int values_dtype, const int64_t *indices, const float *log_rest,

@@ -153,6 +153,16 @@ Loss run_distill(const Tensor &logits, const Inputs &in, bool want_grad) {
 
 std::optional<Tensor> some(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
+// What a backward needs beside the saved inputs, in one value: each entry of a
+// context's dictionary costs a step about a microsecond of host time.
+struct State : public torch::CustomClassHolder {
+    Tensor grad;       // undefined once a backward has handed it over
+    Tensor workspace;  // of the call that wrote grad, where tropnn_hip_distill_grad asks for it
+    Tensor unit;
+    double temperature = 1.0, scale = 1.0;
+    bool mean = true;
+};
+
 struct DistillFunction : public torch::autograd::Function<DistillFunction> {
     // unit: the tensor of one that a training loop may start its backward with
     static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &values, const Tensor &indices,
@@ -162,23 +172,15 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         const Inputs in(logits, values, indices, log_rest, weights, temperature, scale, mean);
         Loss out = run_distill(logits, in, true);
         ctx->save_for_backward({logits, values, indices, log_rest.value_or(Tensor()), weights.value_or(Tensor())});
-        ctx->saved_data["grad"] = std::move(out.grad);
-        if (in.dtype != TROPNN_LOGITS_F32) ctx->saved_data["workspace"] = std::move(out.workspace);
-        ctx->saved_data["temperature"] = temperature;
-        ctx->saved_data["scale"] = scale;
-        ctx->saved_data["mean"] = mean;
-        if (unit.has_value()) ctx->saved_data["unit"] = *unit;
+        auto state = c10::make_intrusive<State>();
+        state->grad = std::move(out.grad);
+        if (in.dtype != TROPNN_LOGITS_F32 && mean && weights.has_value()) state->workspace = std::move(out.workspace);
+        if (unit.has_value()) state->unit = *unit;
+        state->temperature = temperature;
+        state->scale = scale;
+        state->mean = mean;
+        ctx->saved_data["state"] = c10::IValue::make_capsule(std::move(state));
         return out.loss;
-    }
-
-    // A tensor of the context's own, which it then no longer has; undefined
-    // where it has none.
-    static Tensor take(AutogradContext *ctx, const char *name) {
-        const auto it = ctx->saved_data.find(name);
-        if (it == ctx->saved_data.end()) return Tensor();
-        Tensor t = it->second.toTensor();
-        ctx->saved_data.erase(it);
-        return t;
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grad_outputs) {
@@ -190,12 +192,10 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0];
         const c10::DeviceGuard guard(logits.device());
-        bool one = false;  // known on the host
-        if (auto it = ctx->saved_data.find("unit"); it != ctx->saved_data.end()) {
-            const Tensor unit = it->second.toTensor();
-            one = unit._version() == 0 && unit.const_data_ptr() == incoming.const_data_ptr();
-        }
-        Tensor grad = take(ctx, "grad"), workspace = take(ctx, "workspace");
+        const auto state = c10::static_intrusive_pointer_cast<State>(ctx->saved_data["state"].toCapsule());
+        const Tensor &unit = state->unit;
+        const bool one = unit.defined() && unit._version() == 0 && unit.const_data_ptr() == incoming.const_data_ptr();
+        Tensor grad = std::move(state->grad), workspace = std::move(state->workspace);
         if (!(grad.defined() && one)) {
             const Tensor factor = incoming.to(at::kFloat).contiguous();
             const float *f = factor.const_data_ptr<float>();
@@ -205,13 +205,10 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
                       "tropnn_hip_scale_in_place");
             } else {
                 const Inputs in(logits, saved[1], saved[2], some(saved[3]), some(saved[4]),
-                                ctx->saved_data["temperature"].toDouble(), ctx->saved_data["scale"].toDouble(),
-                                ctx->saved_data["mean"].toBool());
+                                state->temperature, state->scale, state->mean);
                 const bool holds = grad.defined();
-                if (!holds) {
-                    grad = at::empty(logits.sizes(), logits.options());
-                    workspace = in.workspace();
-                }
+                if (!holds) grad = at::empty(logits.sizes(), logits.options());
+                if (!workspace.defined()) workspace = in.workspace();
                 in.call("tropnn_hip_distill_grad", g_logits_abi.distill_grad, workspace, f, static_cast<int>(holds),
                         grad.mutable_data_ptr());
             }
