@@ -224,3 +224,19 @@ def test_abi_refuses_bad_arguments_of_the_scaled_gradient(lib):
     none = list(good)
     none[0], none[3] = 0, None
     assert fn(*none) == 0
+
+
+def test_committed_profiles_match_the_kernel_sources():
+    """profiles/logits_*.md name the digest of the kernel sources, comments
+    aside, that they were made from."""
+    import hashlib
+
+    root = HEADER.parent.parent
+    h = hashlib.sha256()
+    for name in ("distill.hip", "select.hip", "logits.hpp"):
+        text = re.sub(r"/\*.*?\*/", " ", (root / "tropnn_amd" / "csrc" / name).read_text(), flags=re.S)
+        h.update(" ".join(re.sub(r"//[^\n]*", " ", text).split()).encode())
+    profiles = sorted((root / "profiles").glob("logits_*.md"))
+    assert [p.stem for p in profiles] == ["logits_counters", "logits_kernel_trace"]
+    for p in profiles:
+        assert h.hexdigest() in p.read_text(), f"{p.name} was made from other kernel sources"

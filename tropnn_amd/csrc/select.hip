@@ -709,7 +709,7 @@ struct TopKernelArgs {
 
 // The row is read once, and the k entries once more (they are in the caches):
 // a row of 4096 x 131072 bf16, k = 64, costs its exponentials and comparisons
-// as much as its bytes: 215 us for 1.07 GB (5 TB/s) with the vector units 74 %
+// as much as its bytes: 215 us for 1.07 GB (5 TB/s) with the vector units 76 %
 // busy, where a reading rate of 6.7 TB/s would take 160. Of few rows, the chain
 // of the bound, the list and its sorting is left: 8 rows take 10 us of 1024
 // logits, 12 of 16384 and 15 of 65536. Exponentials are taken around the bound, known before
