@@ -123,7 +123,10 @@ int tropnn_hip_preference(int64_t pairs, int64_t length, const int64_t *tokens, 
  *   x = (x ^ x >> 15) * 0x3C6EF373;       x = x ^ x >> 16          (mod 2^32)
  * the low 16 bits decide for m, the high ones for u, so the expected value is
  * the f32 one (to 2^-17 of a step). A u above 0 becomes no 0; what is not finite
- * becomes NaN. Zero bytes are a state of zeros.
+ * becomes NaN. A u of NaN counts as infinite: an element whose gradient's square is
+ * past f32 (from 1.85e19 on) takes no step, then and from then on, while m is
+ * finite; an infinite or NaN gradient makes its parameter NaN. The root may be the
+ * f32 beside the nearest. Zero bytes are a state of zeros.
  * params, grads, exp_avgs, exp_avg_exponents, roots, root_exponents, steps: HOST
  * arrays of n_tensors DEVICE pointers: numels[k] f32 (4-byte aligned) for the
  * first two, numels[k] bytes for the codes, (numels[k] + 31) / 32 bytes for the

@@ -476,3 +476,50 @@ def test_a_tensor_past_one_grid_and_32_bits():
     assert int(torch.count_nonzero(p.detach()[2000:1 << 20])) == 0
     del p, opt, state
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("cls,decay", [(FusedAdamW, 0.05), (FusedAdamW, 0.0), (FusedAdam, 0.1)])
+def test_gradients_whose_squares_leave_f32(cls, decay):
+    """From 1.85e19 on a gradient's square is infinite, and so is the root: the
+    element takes no step beyond its decay, neither then nor later, as with 32
+    bits (whose squares go on to 5.8e20). Looked at after the very step. An
+    infinite gradient has no quotient, and neither has a NaN."""
+    sizes = [1e17, 1e18, 1e19, 1.8e19, 1.9e19, 2e19, 1e20, 1e21, 1e25, 3e38, math.inf, math.nan]
+    lr, b1, b2, eps = 1e-2, 0.9, 0.999, 1e-8
+    gradients = torch.randn(2 * len(sizes), BLOCK, generator=torch.Generator().manual_seed(1))
+    gradients[:, 5] = torch.tensor([s * v for v in sizes for s in (1.0, -1.0)])  # one in a block
+    gradients = gradients.flatten()
+    before = torch.linspace(-2, 2, len(gradients))
+    p, q = (torch.nn.Parameter(before.to(DEV)) for _ in range(2))
+    p.grad, q.grad = gradients.to(DEV), gradients.to(DEV)
+    opt = cls([p], lr=lr, weight_decay=decay, state_bits=8)
+    twin = cls([q], lr=lr, weight_decay=decay)
+    opt.step()
+    twin.step()
+    kept, g = before.double(), gradients
+    if cls is FusedAdamW:
+        kept = kept * (1 - lr * decay)
+    else:
+        g = gradients + decay * before
+    root = torch.sqrt((g * g).double() * (1 - b2))
+    want = kept - lr / (1 - b1) * ((1 - b1) * g.double()) / (root / math.sqrt(1 - b2) + eps)
+    infinite = torch.isinf(root) & torch.isfinite(g)
+    assert int(infinite.sum()) == 12 and torch.equal(want[infinite], kept[infinite])
+    got = p.detach().cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and int(torch.isnan(want).sum()) == 4
+    # the decay and the step are roundings of p and of the step, which is lr at most
+    off = (got - want).abs() - U * (4 * before.abs() + 32 * lr)
+    assert (off.nan_to_num(0.0) <= 0).all(), off
+    alike = (g.abs() < 1e19) | (g.abs() > 6e20) | torch.isnan(g)
+    assert torch.allclose(p.detach().cpu()[alike], q.detach().cpu()[alike], rtol=8 * U, atol=U * 32 * lr, equal_nan=True)
+    state = opt.state[p]
+    assert torch.equal(torch.isnan(state["root_8bit"].float().cpu()), infinite | ~torch.isfinite(g))
+    assert torch.equal(torch.isnan(state["exp_avg_8bit"].float().cpu()), ~torch.isfinite(g))
+    for step in range(3):
+        held = p.detach().cpu().double()
+        give_gradients([p], 20 + step)
+        opt.step()
+        want = held * (1 - lr * decay) if cls is FusedAdamW else held
+        got = p.detach().cpu().double()
+        assert ((got - want).abs() <= 2 * U * held.abs())[infinite].all(), step
+        assert torch.equal(torch.isnan(got), ~torch.isfinite(g)), step

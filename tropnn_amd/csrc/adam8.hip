@@ -106,10 +106,13 @@ __device__ __forceinline__ uint32_t random_of(uint32_t x) {
     return x ^ x >> 16;
 }
 
-// Square roots of numbers that are not negative, to the nearest f32: an
-// approximate reciprocal root and one step with the residual, which an fma has
-// exactly. Numbers below 2^-100, whose residual would leave f32, are rare and
-// taken by the library's form.
+// Square roots of numbers that are not negative: an approximate reciprocal root and
+// one Newton step whose residual an fma has exactly (Markstein's sequence). With
+// a reciprocal root that is off by a unit in the last place, 4 of the 16.8 million
+// f32 in [1, 4) get the one beside the nearest. Numbers below 2^-100, whose residual
+// would leave f32, are rare and taken by the library's form. So is infinity, of
+// which the sequence makes a NaN, and so is NaN, which counts as infinity: a root
+// past f32 is held as NaN, and a gradient of NaN makes the first moment NaN too.
 __device__ __forceinline__ void roots_of(float (&x)[kEach]) {
     float root[kEach];
     uint32_t least = ~0u;
@@ -120,9 +123,10 @@ __device__ __forceinline__ void roots_of(float (&x)[kEach]) {
         root[i] = fmaf(fmaf(-s, s, x[i]), 0.5f * y, s);
         least = min(least, __builtin_bit_cast(uint32_t, x[i]) - 1u);  // 0 comes last
     }
-    if (__any(least < __builtin_bit_cast(uint32_t, 0x1p-100f))) {
+    const float all = (root[0] + root[1]) + (root[2] + root[3]);  // finite, or one of them is NaN
+    if (__any(least < __builtin_bit_cast(uint32_t, 0x1p-100f) || all != all)) {
 #pragma unroll 1
-        for (int i = 0; i < kEach; ++i) root[i] = x[i] < 0x1p-100f ? sqrtf(x[i]) : root[i];
+        for (int i = 0; i < kEach; ++i) root[i] = !(x[i] < INFINITY) ? INFINITY : x[i] < 0x1p-100f ? sqrtf(x[i]) : root[i];
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) x[i] = root[i];
@@ -152,9 +156,9 @@ __device__ __forceinline__ uint32_t signs_of(const float (&v)[kEach]) {
 }
 
 // element: of the tensor, the first one; mixed: the step's share of the random
-// numbers. m and u are formed by the operations that the header names, each
-// rounded by itself, so that their exponents do not hang on the compiler; the
-// parameter's quotient is to two units in the last place.
+// numbers. m and the square of u are formed by the operations that the header names,
+// each rounded by itself, so that their exponents do not hang on the compiler; u's
+// root is as above, and the parameter's quotient is to two units in the last place.
 __device__ __forceinline__ void step_elements(Elements &e, const KernelArgs &a, float2 scalars, uint32_t element, uint32_t mixed) {
 #pragma clang fp contract(off)
     float m[kEach], u[kEach];
@@ -173,7 +177,7 @@ __device__ __forceinline__ void step_elements(Elements &e, const KernelArgs &a, 
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         // a denominator below the least normal number, which has no reciprocal here, counts as that
-        const float denominator = fmaxf(fmaf(u[i], scalars.y, a.eps), 0x1p-126f);
+        const float denominator = fmaxf(fmaf(u[i], scalars.y, a.eps), 0x1p-126f);  // a root is no NaN
         e.p[i] = fmaf(-scalars.x, m[i] * __builtin_amdgcn_rcpf(denominator), e.p[i] * a.decay);
     }
     e.m_exp = exponent_of(block_most(m));

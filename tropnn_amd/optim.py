@@ -116,8 +116,9 @@ class FusedAdam(torch.optim.Optimizer):
     "exp_avg_8bit" and "root_8bit" (float8_e4m3fn, the parameter's shape) with
     "exp_avg_exponents" and "root_exponents" (uint8, one for every 32 elements in
     memory order; an element's value is its code times 2^(exponent - 127), and
-    the root is that of exp_avg_sq). A group of a loaded state dict has the
-    state_bits that it was saved with."""
+    the root is that of exp_avg_sq). A root past f32 (of a gradient from 1.85e19 on)
+    is NaN and stands for infinity: its element takes no more steps, as with 32 bits.
+    A group of a loaded state dict has the state_bits that it was saved with."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.0, decoupled_weight_decay: bool = False, *, amsgrad: bool = False,
