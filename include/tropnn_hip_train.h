@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define TROPNN_HIP_TRAIN_ABI_VERSION 1
+#define TROPNN_HIP_TRAIN_ABI_VERSION 2
 
 /* elements of an 8-bit state that share an exponent byte */
 #define TROPNN_STATE_BLOCK 32
@@ -71,10 +71,12 @@ int tropnn_hip_token_gradient(int64_t rows, int64_t vocab, int64_t row_stride, c
  * (the last term only where ref_log_probs is not NULL and kl_weight is not 0).
  * loss[0] = scale * sum_r w_r L_r / D, D = sum of w_r over the rows with a
  * token (mean != 0) or 1; weights NULL: all ones. All arrays f32 [rows].
- * Written: log_probs [rows]; coefs [rows], w_r scale dL/dlp; norm [1], D; stats
- * [rows][2]; so that tropnn_hip_token_gradient(coefs, rows_per_coef 1, norm)
- * gives d loss / d logits. grad (NULL: not wanted) is that gradient, rounded
- * once; it can be had where tropnn_hip_policy_grad_fits says so.
+ * Written: log_probs [rows]; coefs [rows], w_r scale dL/dlp / 2^j; norm [1], D /
+ * 2^j, with j such that norm is from 1/2 to 1 (0 where D is 0 or not finite): a
+ * term may be past f32 where its share of the mean is not; stats [rows][2]; so that
+ * tropnn_hip_token_gradient(coefs, rows_per_coef 1, norm) gives d loss / d logits.
+ * grad (NULL: not wanted) is that gradient, rounded once; it can be had where
+ * tropnn_hip_policy_grad_fits says so.
  */
 int tropnn_hip_policy_grad_fits(int64_t rows, int64_t vocab, int dtype);
 size_t tropnn_hip_policy_workspace_size(int64_t rows, int64_t vocab, int dtype, int want_grad);
@@ -94,9 +96,9 @@ int tropnn_hip_policy(int64_t rows, int64_t vocab, int64_t row_stride, const voi
  * loss[0] = scale * sum_p w_p L_p / D, D = sum w_p (mean != 0) or 1. Pairs of
  * weight 0 take no part, whatever they hold. reference f32 [2][pairs] (NULL:
  * zeros), weights f32 [pairs] (NULL: ones). Written: log_probs f32 [2][pairs],
- * S; coefs f32 [2][pairs], w scale dL / d(a token's log-probability); norm [1],
- * D; so that tropnn_hip_token_gradient(coefs, rows_per_coef length, norm) gives
- * d loss / d logits.
+ * S; coefs f32 [2][pairs], w scale dL / d(a token's log-probability) / 2^j; norm
+ * [1], D / 2^j, with j as above; so that tropnn_hip_token_gradient(coefs,
+ * rows_per_coef length, norm) gives d loss / d logits.
  */
 size_t tropnn_hip_preference_workspace_size(int64_t pairs, int64_t length);
 int tropnn_hip_preference(int64_t pairs, int64_t length, const int64_t *tokens, const double *token_log_probs,

@@ -13,7 +13,7 @@ import torch
 from .logits_hip import load_logits_library
 from .pairwise_hip import _LOCK, _pairwise_op, library_path
 
-TRAIN_ABI_VERSION = 1
+TRAIN_ABI_VERSION = 2
 STATE_BLOCK = 32  # elements of an 8-bit state that share an exponent
 
 TRAIN_SYMBOLS = (

@@ -306,12 +306,24 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms &a, int64_t ro
     return t;
 }
 
+// What a mean divides by, the sum of the weights, as a number from 1/2 to 1 and a
+// power of two. What it divides is divided by the power in f64, before f32 holds it:
+// the one coefficient of a mean over many rows may be past f32 where its share of
+// the mean is not, and so may the sum be.
+struct Norm {
+    double sum;
+    int power;  // 0 where the sum is 0 or not finite
+
+    __device__ __forceinline__ explicit Norm(double by) : sum(by), power(__builtin_amdgcn_frexp_exp(by)) {}
+    __device__ __forceinline__ float of(double v) const { return static_cast<float>(__builtin_amdgcn_ldexp(v, -power)); }
+    __device__ __forceinline__ float fraction() const { return of(sum); }
+};
+
 struct ScoreKernelArgs {
     ScoreArgs s;
     int64_t first_row;
     PolicyTerms terms;  // old_log_probs NULL: the log-probabilities alone
-    double *row_loss;
-    float *coefs;
+    double *row_loss, *row_by;  // weighted, and the scale's product with the latter
 };
 
 __device__ __forceinline__ void store_log_prob(const ScoreArgs &a, int64_t row, double log_prob) {
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(THREADS) void token_score_kernel(ScoreKernelArgs a)
         // no part of a loss; a weighted row's log-probability is still wanted
         if (tid == 0 && a.row_loss) {
             a.row_loss[row] = 0.0;
-            a.coefs[row] = 0.f;
+            a.row_by[row] = 0.0;
         }
         if (token < 0) {
             if (tid == 0) store_log_prob(a.s, row, 0.0);
@@ -375,7 +387,7 @@ __global__ __launch_bounds__(THREADS) void token_score_kernel(ScoreKernelArgs a)
     if (a.row_loss && weight != 0.f) {
         const PolicyRow p = policy_row(a.terms, row, t.log_prob);
         a.row_loss[row] = static_cast<double>(weight) * p.loss;
-        a.coefs[row] = static_cast<float>(static_cast<double>(weight) * a.terms.scale * p.by);
+        a.row_by[row] = static_cast<double>(weight) * a.terms.scale * p.by;
     }
 }
 
@@ -451,7 +463,7 @@ struct HeldArgs {
     ScoreArgs s;
     int64_t first_row;
     PolicyTerms terms;
-    const RowSums *parts;  // of the weights, whose sum divides the loss; NULL: nothing does
+    const RowSums *parts;  // of the weights, whose sum divides the loss; NULL: 1 does
     int n_parts;
     double *row_loss;
     float *coefs;
@@ -529,8 +541,9 @@ __global__ __launch_bounds__(THREADS) void policy_held_kernel(HeldArgs a) {
         g.l = t.l;
         PolicyRow p{0.0, 0.0};
         if (weight != 0.f) p = policy_row(a.terms, row, t.log_prob);
-        const float coef = static_cast<float>(static_cast<double>(weight) * a.terms.scale * p.by);
-        g.by = coef == 0.f ? 0.f : coef / static_cast<float>(norm) / a.s.temper.t;
+        const Norm by(norm);
+        const float coef = by.of(static_cast<double>(weight) * a.terms.scale * p.by);
+        g.by = coef == 0.f ? 0.f : coef / by.fraction() / a.s.temper.t;
         g.at_token = g.by == 0.f ? 0.f : -g.by * expm1f(fmaf(x_a - t.ref, r.c, -t.l) * kLn2);  // the row may hold anything
         if (tid == 0) {
             store_log_prob(a.s, row, t.log_prob);
@@ -588,22 +601,53 @@ struct TotalArgs {
     bool mean;
     RowSums *parts;
     float *loss, *norm;  // loss NULL: the parts alone
+    const double *by;    // what the mean divides beside the loss, and
+    float *coefs;        // where it goes; n_coefs 0: nothing
+    int64_t n_coefs;
 };
 
-__device__ __forceinline__ void store_total(const TotalArgs &a, RowSums s) {
-    const double norm = a.mean ? s.weight : 1.0;
-    *a.norm = static_cast<float>(norm);
-    *a.loss = static_cast<float>(a.scale * s.loss / norm);
+__device__ __forceinline__ Norm norm_of(const TotalArgs &a, const RowSums &s) { return Norm(a.mean ? s.weight : 1.0); }
+
+__device__ __forceinline__ void store_total(const TotalArgs &a, const RowSums &s) {
+    const Norm norm = norm_of(a, s);
+    *a.norm = norm.fraction();
+    *a.loss = static_cast<float>(a.scale * s.loss / norm.sum);
 }
 
+// Coefficients of one workgroup, eight of a thread in flight: loaded before the norm
+// is known, stored after that.
+struct Coefs {
+    static constexpr int U = 8;
+    double by[U];
+
+    __device__ __forceinline__ void load(const TotalArgs &a, int64_t first) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = first + u * kSumThreads + threadIdx.x;
+            by[u] = i < a.n_coefs ? a.by[i] : 0.0;
+        }
+    }
+    __device__ __forceinline__ void store(const TotalArgs &a, const Norm &norm, int64_t first) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = first + u * kSumThreads + threadIdx.x;
+            if (i < a.n_coefs) a.coefs[i] = norm.of(by[u]);
+        }
+    }
+};
+constexpr int64_t kSumRows = int64_t{Coefs::U} * kSumThreads;
+
 // Sums over a run of rows per workgroup, in a fixed order; one workgroup of all
-// rows finishes the loss. Eight loads of each array are in flight: one workgroup
-// takes 8192 rows in a round trip to memory.
+// rows finishes the loss and the coefficients. Eight loads of each array are in
+// flight: one workgroup takes 8192 rows in a round trip to memory.
 __global__ __launch_bounds__(kSumThreads) void total_kernel(TotalArgs a) {
     __shared__ RowSums scratch[kSumThreads / kWave];
     constexpr int U = 8;
     const int64_t each = ((a.rows + gridDim.x - 1) / gridDim.x + kSumThreads - 1) / kSumThreads * kSumThreads;
     const int64_t end = min(each * (blockIdx.x + 1), a.rows);
+    const bool alone = a.loss && gridDim.x == 1;
+    Coefs coefs;
+    if (alone) coefs.load(a, 0);
     RowSums sum{0.0, 0.0};
     for (int64_t first = each * blockIdx.x; first < end; first += U * kSumThreads) {
         int64_t token[U];
@@ -624,24 +668,45 @@ __global__ __launch_bounds__(kSumThreads) void total_kernel(TotalArgs a) {
         }
     }
     sum = workgroup_sums(sum, scratch);
-    if (threadIdx.x != 0) return;
-    a.parts[blockIdx.x] = sum;
-    if (a.loss && gridDim.x == 1) store_total(a, sum);
+    if (threadIdx.x == 0) a.parts[blockIdx.x] = sum;
+    if (!alone) return;
+    if (threadIdx.x == 0) store_total(a, sum);
+    if (a.n_coefs == 0) return;
+    __shared__ double weight;
+    if (threadIdx.x == 0) weight = sum.weight;
+    __syncthreads();
+    const Norm norm = norm_of(a, RowSums{0.0, weight});
+    coefs.store(a, norm, 0);
+    for (int64_t first = kSumRows; first < a.n_coefs; first += kSumRows) {
+        coefs.load(a, first);
+        coefs.store(a, norm, first);
+    }
 }
 
-// The loss from several workgroups' sums.
-__global__ __launch_bounds__(kWave) void join_kernel(TotalArgs a, int parts) {
-    const bool in = static_cast<int>(threadIdx.x) < parts;
-    RowSums s = in ? a.parts[threadIdx.x] : RowSums{0.0, 0.0};
+// The loss from several workgroups' sums, which every wave adds up for itself, and
+// the coefficients, a run of them per workgroup at a time.
+__global__ __launch_bounds__(kSumThreads) void join_kernel(TotalArgs a, int parts) {
+    Coefs coefs;
+    int64_t first = blockIdx.x * kSumRows;
+    coefs.load(a, first);
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    RowSums s = lane < parts ? a.parts[lane] : RowSums{0.0, 0.0};
     s.loss = wave_add(s.loss);
     s.weight = wave_add(s.weight);
-    if (threadIdx.x == 0) store_total(a, s);
+    if (blockIdx.x == 0 && threadIdx.x == 0) store_total(a, s);
+    const Norm norm = norm_of(a, s);
+    while (first < a.n_coefs) {
+        coefs.store(a, norm, first);
+        first += gridDim.x * kSumRows;
+        coefs.load(a, first);
+    }
 }
 
 constexpr int kPairThreads = 256;
 
 // A pair of sequences per workgroup.
-__global__ __launch_bounds__(kPairThreads) void preference_kernel(PreferenceArgs a, int64_t first_pair, double *pair_loss) {
+__global__ __launch_bounds__(kPairThreads) void preference_kernel(PreferenceArgs a, int64_t first_pair, double *pair_loss,
+                                                                  double *pair_by) {
     __shared__ RowSums scratch[2][kPairThreads / kWave];
     const int64_t pair = first_pair + blockIdx.x;
     RowSums part[2] = {{0.0, 0.0}, {0.0, 0.0}};  // of log-probabilities, and how many
@@ -684,8 +749,8 @@ __global__ __launch_bounds__(kPairThreads) void preference_kernel(PreferenceArgs
         by = a.beta * (sigmoid_minus_one + smoothing);
     }
     pair_loss[pair] = weight * loss;
-    a.coefs[pair] = static_cast<float>(weight * by * share[0] * a.scale);
-    a.coefs[a.pairs + pair] = static_cast<float>(-weight * by * share[1] * a.scale);
+    pair_by[pair] = weight * by * share[0] * a.scale;
+    pair_by[a.pairs + pair] = -weight * by * share[1] * a.scale;
 }
 
 template <typename T, int THREADS, int U, bool NT = false>
@@ -745,15 +810,22 @@ hipError_t launch_gradient(GradKernelArgs k, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// One workgroup up to 64 K rows, then more, at most a wave's lanes.
-int sum_parts(int64_t rows) { return static_cast<int>(rows <= 65536 ? 1 : rows < 65536 * 64 ? (rows + 65535) / 65536 : 64); }
+// One workgroup up to two round trips of rows, then one for each, at most a wave's
+// lanes. 16000 rows take one workgroup 13.6 us, two and the launch that joins them
+// 9.7, but a launch costs the host 3 (a call with its gradient 64 to 67 us and
+// 67.5); 65536 take eight and a join 10.8, one 41.
+int sum_parts(int64_t rows) {
+    return static_cast<int>(rows <= 2 * kSumRows ? 1 : std::min<int64_t>((rows + kSumRows - 1) / kSumRows, kWave));
+}
 
 hipError_t launch_total(const TotalArgs &a, hipStream_t stream) {
     const int parts = sum_parts(a.rows);
     hipLaunchKernelGGL(total_kernel, dim3(static_cast<uint32_t>(parts)), dim3(kSumThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (parts == 1 || !a.loss) return hipSuccess;
-    hipLaunchKernelGGL(join_kernel, dim3(1), dim3(kWave), 0, stream, a, parts);
+    const int64_t runs = std::min<int64_t>((a.n_coefs + kSumRows - 1) / kSumRows, 4 * kCus);
+    hipLaunchKernelGGL(join_kernel, dim3(static_cast<uint32_t>(std::max<int64_t>(runs, 1))), dim3(runs > 0 ? kSumThreads : kWave), 0,
+                       stream, a, parts);
     return hipGetLastError();
 }
 
@@ -817,21 +889,28 @@ bool policy_grad_fits(const LogitRows &x) {
 
 namespace {
 
-// A loss per row or pair, then the sums' parts.
-size_t losses_bytes(int64_t n) { return (sizeof(double) * static_cast<size_t>(n) + 15) / 16 * 16; }
-RowSums *parts_of(void *workspace, int64_t n) { return reinterpret_cast<RowSums *>(static_cast<char *>(workspace) + losses_bytes(n)); }
+// A loss per row or pair, the sums' parts, and what becomes coefficients.
+struct Losses {
+    size_t parts, by, bytes;  // where they begin, and the end
+
+    Losses(int64_t n, int64_t coefs)
+        : parts((sizeof(double) * static_cast<size_t>(n) + 15) / 16 * 16),
+          by(parts + sizeof(RowSums) * static_cast<size_t>(sum_parts(n))), bytes(by + sizeof(double) * static_cast<size_t>(coefs)) {}
+};
 
 }  // namespace
 
-size_t policy_workspace(const LogitRows &x, bool) {
-    return losses_bytes(x.rows) + sizeof(RowSums) * static_cast<size_t>(sum_parts(x.rows));
-}
+// A forward that writes the gradient knows the norm before its coefficients.
+size_t policy_workspace(const LogitRows &x, bool want_grad) { return Losses(x.rows, want_grad ? 0 : x.rows).bytes; }
 
 hipError_t launch_policy(const PolicyArgs &a, void *workspace, hipStream_t stream) {
     const LogitRows &x = a.score.x;
-    double *row_loss = static_cast<double *>(workspace);
-    RowSums *parts = parts_of(workspace, x.rows);
-    TotalArgs t{nullptr, a.score.tokens, a.terms.weights, x.rows, a.terms.scale, a.mean, parts, nullptr, a.norm};
+    const Losses at(x.rows, a.grad ? 0 : x.rows);
+    char *const ws = static_cast<char *>(workspace);
+    double *const row_loss = reinterpret_cast<double *>(ws), *const row_by = reinterpret_cast<double *>(ws + at.by);
+    RowSums *const parts = reinterpret_cast<RowSums *>(ws + at.parts);
+    TotalArgs t{nullptr, a.score.tokens, a.terms.weights, x.rows, a.terms.scale, a.mean, parts, nullptr, a.norm,
+                row_by, a.coefs, a.grad ? 0 : x.rows};
     if (a.grad && x.rows > 0) {
         if (a.mean) {
             if (hipError_t e = launch_total(t, stream); e != hipSuccess) return e;
@@ -840,24 +919,26 @@ hipError_t launch_policy(const PolicyArgs &a, void *workspace, hipStream_t strea
         hipError_t e = with_logit_type(x.dtype, [&](auto t) { return launch_held_by_width<decltype(t)>(k, stream); });
         if (e != hipSuccess) return e;
     } else if (x.rows > 0) {
-        if (hipError_t e = launch_scores(ScoreKernelArgs{a.score, 0, a.terms, row_loss, a.coefs}, stream); e != hipSuccess) return e;
+        if (hipError_t e = launch_scores(ScoreKernelArgs{a.score, 0, a.terms, row_loss, row_by}, stream); e != hipSuccess) return e;
     }
     t.row_loss = row_loss;
     t.loss = a.loss;
     return launch_total(t, stream);
 }
 
-size_t preference_workspace(int64_t pairs, int64_t) {
-    return losses_bytes(pairs) + sizeof(RowSums) * static_cast<size_t>(sum_parts(pairs));
-}
+size_t preference_workspace(int64_t pairs, int64_t) { return Losses(pairs, 2 * pairs).bytes; }
 
 hipError_t launch_preference(const PreferenceArgs &a, void *workspace, hipStream_t stream) {
-    double *pair_loss = static_cast<double *>(workspace);
+    const Losses at(a.pairs, 2 * a.pairs);
+    char *const ws = static_cast<char *>(workspace);
+    double *const pair_loss = reinterpret_cast<double *>(ws), *const pair_by = reinterpret_cast<double *>(ws + at.by);
     hipError_t e = by_grids(a.pairs, [&](int64_t first, uint32_t pairs) {
-        hipLaunchKernelGGL(preference_kernel, dim3(pairs), dim3(kPairThreads), 0, stream, a, first, pair_loss);
+        hipLaunchKernelGGL(preference_kernel, dim3(pairs), dim3(kPairThreads), 0, stream, a, first, pair_loss, pair_by);
     });
     if (e != hipSuccess) return e;
-    return launch_total(TotalArgs{pair_loss, nullptr, a.weights, a.pairs, a.scale, a.mean, parts_of(workspace, a.pairs), a.loss, a.norm}, stream);
+    return launch_total(TotalArgs{pair_loss, nullptr, a.weights, a.pairs, a.scale, a.mean, reinterpret_cast<RowSums *>(ws + at.parts),
+                                  a.loss, a.norm, pair_by, a.coefs, 2 * a.pairs},
+                        stream);
 }
 
 }  // namespace tropnn
