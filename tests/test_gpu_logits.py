@@ -1074,3 +1074,48 @@ def test_sample_against_64_bits_with_wide_gaps(vocab, dtype, kw):
     assert (p[ok] > 0).all()
     assert ((u.double() <= high + 3e-5) & (u.double() >= high - p - 3e-5))[ok].all()
     assert torch.allclose(got.log_probs.cpu().double()[ok], p[ok].log(), rtol=REL, atol=REL)
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_distillation_backward_captured_apart_from_its_forward(dtype, weighted):
+    """A backward in a graph of its own writes its gradient in every replay,
+    whatever the factor and whatever became of the last one; one that its
+    forward's graph holds too does so as well."""
+    rows, vocab = 70, 900
+    logits = rows_of(rows, vocab, dtype, 1)
+    values, indices, log_rest = make_record(rows, vocab, 9, 2)
+    weights = torch.linspace(0.0, 2.0, rows, device=DEV) if weighted else None
+    factor = torch.ones((), device=DEV)
+
+    def forward(x):
+        return distillation_loss(x, values, indices, log_rest, weights=weights)
+
+    def eager(by):
+        x = logits.detach().requires_grad_(True)
+        return torch.autograd.grad(forward(x), x, torch.full((), by, device=DEV))[0]
+
+    eager(1.0)
+    first, second, both = (torch.cuda.CUDAGraph() for _ in range(3))
+    side = torch.cuda.Stream(DEV)
+    x = logits.detach().requires_grad_(True)
+    with torch.cuda.graph(first, stream=side):
+        loss = forward(x)
+    with torch.cuda.graph(second, pool=first.pool(), stream=side):
+        (grad,) = torch.autograd.grad(loss, x, factor)
+    y = logits.detach().requires_grad_(True)
+    with torch.cuda.graph(both, stream=side):
+        (together,) = torch.autograd.grad(forward(y), y, factor)
+    # computed again or scaled where it was written: a rounding apart
+    close = dict(rtol=4 * HALF_ULP[dtype], atol=2 * SMALLEST[dtype])
+    for rep in range(2):
+        logits.copy_(rows_of(rows, vocab, dtype, 20 + rep))
+        first.replay()
+        for by in (1.0, 0.5, 1.0, -2.0):
+            factor.fill_(by)
+            second.replay()
+            both.replay()
+            want = eager(by).float()
+            assert torch.allclose(grad.float(), want, **close) and torch.allclose(together.float(), want, **close), (rep, by)
+            grad.mul_(3.0)
+            together.mul_(3.0)

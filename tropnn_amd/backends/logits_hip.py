@@ -86,7 +86,7 @@ def distill_op() -> Any:
     with _LOCK:
         if _DISTILL_OP is None:
             names = ("tropnn_hip_distill", "tropnn_hip_distill_workspace_size", "tropnn_hip_distill_grad",
-                     "tropnn_hip_scale_in_place", "tropnn_hip_last_error")
+                     "tropnn_hip_scale_in_place", "tropnn_hip_capture_id", "tropnn_hip_last_error")
             torch.ops.tropnn_hip.bind_logits_abi(
                 *(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), LOGITS_ABI_VERSION)
             _DISTILL_OP = torch.ops.tropnn_hip.distill.default

@@ -13,9 +13,11 @@
 // the factor before its rounding: a loss scaled against f16's underflow needs
 // the bits that the unscaled gradient does not have. Either moves as many bytes
 // (a read and a write of the gradient's size). A second backward through the
-// same node computes the gradient again from the saved inputs. The gradient has
-// no derivative of its own: where a graph of the backward is made, it hangs on a
-// node that raises.
+// same node computes the gradient again from the saved inputs, and so does one that
+// is not in the capture of its forward, or in none with it: replayed without the
+// forward it would find what its last replay gave away. The gradient has no
+// derivative of its own: where a graph of the backward is made, it hangs on a node
+// that raises.
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
@@ -33,6 +35,7 @@
 
 #include "op_rows.hpp"
 #include "tropnn_hip_logits.h"
+#include "tropnn_hip_train.h"
 
 namespace {
 
@@ -48,22 +51,25 @@ struct LogitsAbi {
     decltype(&tropnn_hip_distill_workspace_size) distill_workspace_size = nullptr;
     decltype(&tropnn_hip_distill_grad) distill_grad = nullptr;
     decltype(&tropnn_hip_scale_in_place) scale_in_place = nullptr;
+    decltype(&tropnn_hip_capture_id) capture_id = nullptr;
     decltype(&tropnn_hip_last_error) last_error = nullptr;
 };
 LogitsAbi g_logits_abi;
 std::atomic<bool> g_logits_bound{false};
 
 void bind_logits_abi(int64_t distill, int64_t distill_workspace_size, int64_t distill_grad, int64_t scale_in_place,
-                     int64_t last_error, int64_t abi_version) {
+                     int64_t capture_id, int64_t last_error, int64_t abi_version) {
     TORCH_CHECK(abi_version == TROPNN_HIP_LOGITS_ABI_VERSION, "libtropnn_hip.so has logits ABI version ", abi_version,
                 ", the autograd operator was built for ", TROPNN_HIP_LOGITS_ABI_VERSION);
-    TORCH_CHECK(distill != 0 && distill_workspace_size != 0 && distill_grad != 0 && scale_in_place != 0 && last_error != 0,
+    TORCH_CHECK(distill != 0 && distill_workspace_size != 0 && distill_grad != 0 && scale_in_place != 0 && capture_id != 0 &&
+                    last_error != 0,
                 "bind_logits_abi: NULL entry point");
     auto set = [](auto &f, int64_t address) { f = reinterpret_cast<std::decay_t<decltype(f)>>(static_cast<intptr_t>(address)); };
     set(g_logits_abi.distill, distill);
     set(g_logits_abi.distill_workspace_size, distill_workspace_size);
     set(g_logits_abi.distill_grad, distill_grad);
     set(g_logits_abi.scale_in_place, scale_in_place);
+    set(g_logits_abi.capture_id, capture_id);
     set(g_logits_abi.last_error, last_error);
     g_logits_bound.store(true, std::memory_order_release);
 }
@@ -109,6 +115,11 @@ struct Inputs {
     }
 };
 
+// The number of the capture that records the current stream, 0: none does.
+unsigned long long capture_of(const Tensor &t) {
+    return g_logits_abi.capture_id(c10::hip::getCurrentHIPStream(t.device().index()).stream());
+}
+
 struct Loss {
     Tensor loss, grad, workspace;
 };
@@ -130,6 +141,7 @@ std::optional<Tensor> some(const Tensor &t) { return t.defined() ? std::optional
 struct State : public torch::CustomClassHolder {
     Tensor grad;       // undefined once a backward has handed it over
     Tensor workspace;  // of the call that wrote grad, where tropnn_hip_distill_grad asks for it
+    unsigned long long capture = 0;  // that wrote them, 0: none did
     Tensor unit;
     double temperature = 1.0, scale = 1.0;
     bool mean = true;
@@ -146,6 +158,7 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         ctx->save_for_backward({logits, values, indices, log_rest.value_or(Tensor()), weights.value_or(Tensor())});
         auto state = c10::make_intrusive<State>();
         state->grad = std::move(out.grad);
+        state->capture = capture_of(logits);
         if (in.dtype != TROPNN_LOGITS_F32 && mean && weights.has_value()) state->workspace = std::move(out.workspace);
         if (unit.has_value()) state->unit = *unit;
         state->temperature = temperature;
@@ -168,6 +181,10 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         const Tensor &unit = state->unit;
         const bool one = unit.defined() && unit._version() == 0 && unit.const_data_ptr() == incoming.const_data_ptr();
         Tensor grad = std::move(state->grad), workspace = std::move(state->workspace);
+        if (grad.defined() && capture_of(logits) != state->capture) {
+            grad.reset();
+            workspace.reset();
+        }
         if (!(grad.defined() && one)) {
             const Tensor factor = incoming.to(at::kFloat).contiguous();
             const float *f = factor.const_data_ptr<float>();
@@ -211,7 +228,7 @@ Tensor distill(const Tensor &logits, const Tensor &values, const Tensor &indices
 
 TORCH_LIBRARY_FRAGMENT(tropnn_hip, m) {
     m.def("bind_logits_abi(int distill, int distill_workspace_size, int distill_grad, int scale_in_place, "
-          "int last_error, int abi_version) -> ()",
+          "int capture_id, int last_error, int abi_version) -> ()",
           &bind_logits_abi);
     // the layout that distill reads logits in, for any device: (tensor, rows, vocab, row stride)
     m.def("logit_rows(Tensor logits) -> (Tensor, int, int, int)", [](const Tensor &logits) {
