@@ -523,3 +523,21 @@ def test_gradients_whose_squares_leave_f32(cls, decay):
         got = p.detach().cpu().double()
         assert ((got - want).abs() <= 2 * U * held.abs())[infinite].all(), step
         assert torch.equal(torch.isnan(got), ~torch.isfinite(g)), step
+
+
+def test_loading_takes_no_more_memory_than_the_state():
+    n = 1 << 24
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    saved = FusedAdam([p], state_bits=8)
+    saved.state[p] = saved._new_state(p, 8)
+    opt = FusedAdam([p], state_bits=8)
+    state = saved.state_dict()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(DEV)
+    torch.cuda.reset_peak_memory_stats(DEV)
+    opt.load_state_dict(state)
+    # two codes and two sixteenths of a byte an element, and what the allocator rounds up
+    assert torch.cuda.max_memory_allocated(DEV) - before <= n * (2 + 2 / 32) + 4096
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert int(saved.state[p]["root_8bit"].view(torch.uint8).count_nonzero()) == 0

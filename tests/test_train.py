@@ -267,3 +267,38 @@ def test_committed_profiles_match_the_kernel_sources():
     assert [p.stem for p in profiles] == ["train_counters", "train_kernel_trace"]
     for p in profiles:
         assert h.hexdigest() in p.read_text(), f"{p.name} was made from other kernel sources"
+
+
+def test_loading_an_8_bit_state_leaves_its_types_alone():
+    """Hooks around the loading see codes and exponents in their own types: they are
+    never widened, which would take 8 bytes a parameter for a state of 2. What is
+    loaded is the optimizer's own."""
+    opt = with_state(8)
+    saved = opt.state_dict()
+    other = FusedAdam([torch.nn.Parameter(torch.zeros(70))])
+    seen = []
+
+    def note(states):
+        seen.append({key: (t.dtype, t.shape) for s in states for key, t in s.items()})
+
+    handles = (other.register_load_state_dict_pre_hook(lambda o, s: note(s["state"].values())),
+               other.register_load_state_dict_post_hook(lambda o: note(o.state.values())))
+    for _ in range(2):  # the second time over a state
+        other.load_state_dict(saved)
+    for handle in handles:
+        handle.remove()
+    want = next(iter(opt.state.values()))
+    assert seen == [{key: (t.dtype, t.shape) for key, t in want.items()}] * 4
+    got = next(iter(other.state.values()))
+    for key in want:
+        if key != "step":
+            assert got[key].data_ptr() != want[key].data_ptr()
+    # as a tool may have saved it: widened
+    wide = {"param_groups": saved["param_groups"], "state": {0: {k: t.float() for k, t in want.items()}}}
+    other.load_state_dict(wide)
+    got = next(iter(other.state.values()))
+    for key in want:
+        assert got[key].dtype == want[key].dtype and torch.equal(got[key].float(), want[key].float())
+    with pytest.raises(ValueError, match="parameter group"):
+        other.load_state_dict({"param_groups": [], "state": {}})
+    assert not other._optimizer_load_state_dict_pre_hooks and not other._optimizer_load_state_dict_post_hooks

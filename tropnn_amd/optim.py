@@ -107,6 +107,30 @@ _STATE_TYPES = {"exp_avg_8bit": torch.float8_e4m3fn, "root_8bit": torch.float8_e
                 "exp_avg_exponents": torch.uint8, "root_exponents": torch.uint8}
 
 
+class _Kept:
+    """A tensor that torch's loader passes on as it is."""
+
+    def __init__(self, tensor: torch.Tensor) -> None:
+        self.tensor = tensor
+
+
+def _keep_codes(_: torch.optim.Optimizer, state_dict: dict) -> dict:
+    def kept(state):
+        if not isinstance(state, dict):
+            return state
+        return {k: _Kept(v) if k in _STATE_TYPES and isinstance(v, torch.Tensor) else v for k, v in state.items()}
+
+    return {**state_dict, "state": {k: kept(state) for k, state in state_dict["state"].items()}}
+
+
+def _give_codes(optimizer: torch.optim.Optimizer) -> None:
+    for p, state in optimizer.state.items():
+        for key, dtype in _STATE_TYPES.items():
+            if isinstance(state, dict) and isinstance(state.get(key), _Kept):
+                t = state[key].tensor.detach()
+                state[key] = t.to(device=p.device if isinstance(p, torch.Tensor) else t.device, dtype=dtype, copy=True)
+
+
 class FusedAdam(torch.optim.Optimizer):
     """torch.optim.Adam's update (amsgrad=False, maximize=False) on the GPU in
     one launch per parameter group and device. decoupled_weight_decay=True
@@ -149,15 +173,19 @@ class FusedAdam(torch.optim.Optimizer):
         e.g. on the CPU for a torch.optim.Adam state dict or a checkpoint
         loaded with map_location="cpu"; the kernel reads it from the
         parameter's device as f32. It also casts all other state to the
-        parameter's type: codes and exponents get theirs back, which f32 holds
-        exactly. A group saved without state_bits has 32."""
-        super().load_state_dict(state_dict)
+        parameter's type, four times the bytes of codes and exponents: those are
+        kept from it and copied as they are. A group saved without state_bits has
+        32."""
+        hooks = (self.register_load_state_dict_pre_hook(_keep_codes),
+                 self.register_load_state_dict_post_hook(_give_codes, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
         for group in self.param_groups:
             group.setdefault("state_bits", 32)
         for p, state in self.state.items():
-            for key, dtype in _STATE_TYPES.items():
-                if key in state and state[key].dtype != dtype:
-                    state[key] = state[key].to(dtype)
             step = state.get("step")
             if step is None:
                 continue
