@@ -72,7 +72,7 @@ int tropnn_hip_token_gradient(int64_t rows, int64_t vocab, int64_t row_stride, c
  * loss[0] = scale * sum_r w_r L_r / D, D = sum of w_r over the rows with a
  * token (mean != 0) or 1; weights NULL: all ones. All arrays f32 [rows].
  * Written: log_probs [rows]; coefs [rows], w_r scale dL/dlp / 2^j; norm [1], D /
- * 2^j, with j such that norm is from 1/2 to 1 (0 where D is 0 or not finite): a
+ * 2^j, with j such that norm has a size of 1/2 to 1 (j 0 where D is 0 or not finite): a
  * term may be past f32 where its share of the mean is not; stats [rows][2]; so that
  * tropnn_hip_token_gradient(coefs, rows_per_coef 1, norm) gives d loss / d logits.
  * grad (NULL: not wanted) is that gradient, rounded once; it can be had where

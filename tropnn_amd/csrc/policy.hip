@@ -9,8 +9,10 @@
 // s their sum around it and d = (m - x_a) / temperature, the token's log-probability
 // is -(d + log(s + e^-d)), or -log(1 + s e^d) where the token is the largest: full
 // relative precision where it has nearly all of the mass. These few numbers of a row
-// are f64, since a loss may be the small rest of large terms of both signs: 2e-8 of a
-// log-probability at 4096 x 131072 bf16 (3e-7 with all of it in f32, 1% faster).
+// are f64, since a loss may be the small rest of large terms of both signs: 1.5e-8 of a
+// log-probability at 131072 classes (3e-7 with all of it in f32, 1% faster), 3e-8 at
+// ten, where a term's own exponential is the error and the worst of 100000 rows has
+// 1.6e-7.
 // A row's statistics (ref, l) give every class's probability as 2^(c (x_i - ref) - l),
 // and the token's gradient 1 - p_a as 1 - 2^(...) by expm1. Sixteen terms are summed
 // in f32, what they come to and sums over rows and tokens in f64.
@@ -332,8 +334,8 @@ __device__ __forceinline__ void store_log_prob(const ScoreArgs &a, int64_t row, 
 }
 
 // A row per workgroup, streamed, U pieces a thread in flight. Bound by memory:
-// 4096 x 131072 bf16 (1.07 GB) 181 us, 5.9 TB/s; 8192 x 32768 bf16 94 us; a wave
-// per row at 8192 x 512 f32 7.1 us.
+// 4096 x 131072 bf16 (1.07 GB) 159 us past the caches, 6.8 TB/s; 8192 x 32768 bf16 82;
+// a wave per row at 8192 x 512 f32 7.1 us.
 template <typename T, int THREADS, int U, bool NT>
 __global__ __launch_bounds__(THREADS) void token_score_kernel(ScoreKernelArgs a) {
     using R = TokenRow<T, THREADS>;
@@ -861,7 +863,10 @@ hipError_t launch_held(HeldArgs k, hipStream_t stream) {
 
 // As few threads as keep it to eight pieces a thread while several workgroups share
 // a CU: 32768 x 4096 f32 202 us with 256 threads, 207 with 128, 216 with 512; 8192 x
-// 32768 bf16 195 with 512, 210 with 256, 216 with 1024.
+// 32768 bf16 195 with 512, 210 with 256, 216 with 1024. Sixteen a thread before a row
+// fills a CU: 1000 x 50001 f16 60 us with 512 threads, 67 with 1024, 4096 of them 173
+// and 208, 4096 x 65536 bf16 203 and 223 (4096 x 32768 f32, two thirds with a token,
+// 168 and 164).
 template <typename T>
 hipError_t launch_held_by_width(const HeldArgs &k, hipStream_t stream) {
     const int pieces = (k.s.x.vocab + kPerLoad<T> - 1) / kPerLoad<T>;
